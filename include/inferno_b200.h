@@ -39,11 +39,13 @@ extern "C" {
 
 /* ggml type ids accepted (GGUF spec; src/GGUF.jl:25-60) */
 #define INFERNO_F32 0
+#define INFERNO_F16 1   /* long-context operators only */
 #define INFERNO_Q8_0 8
 #define INFERNO_Q4_K 12
 #define INFERNO_Q5_K 13
 #define INFERNO_Q6_K 14
 #define INFERNO_IQ2_XXS 16
+#define INFERNO_BF16 30 /* long-context operators only */
 
 /* thread-local message of the last failing call on this thread */
 const char* inferno_last_error(void);
@@ -172,6 +174,138 @@ int inferno_attention_step(const float* qg, const float* k, const float* v, cons
  * Stream-ordered scratch of about T * n_heads * 1.3 KB. */
 int inferno_gdn_chunked(int T, int n_heads, int dk, int dv, const float* q, const float* k, const float* v,
                         const float* beta, const float* g, float* S, float* y, int chunk, void* stream);
+
+/* ---- long-context serving: rotary positions with cache append, attention
+ * over a shared prefix and per-sequence caches, eviction by gathered weight.
+ * None of the three has a counterpart in the reference, whose attention reads
+ * one contiguous fp32 cache per sequence (src/FlashAttention.jl:16-74); they
+ * work on the same cache layout, a slice [rows][n_kv_heads][head_dim] per
+ * sequence.  `type` is INFERNO_F32, INFERNO_F16 or INFERNO_BF16 and holds for
+ * q, k, v, caches and outputs alike; sums, softmax statistics and gathered
+ * weights are fp32.  Pointers are device pointers of the current device;
+ * struct_size must be sizeof of the struct.  The calls are asynchronous on
+ * `stream`, allocate nothing, can be captured into a graph, and read lengths,
+ * positions and slots on the device only.  A workspace holds nothing between
+ * calls and needs no initialisation; calls that may run at the same time (two
+ * streams, two graphs replayed side by side) need one each. ---- */
+
+/* Rotary positions.  Token t's q (n_heads heads) and k (n_kv_heads heads;
+ * k may be NULL) are rotated by the angles positions[t] * f_i, i < rope_dim / 2,
+ * on the first rope_dim values of each head; the others are copied.  With
+ * slots, token t's rotated k goes to row slots[t] of k_out and its v (if given)
+ * unchanged to row slots[t] of v_out: the append to a cache.  A slot outside
+ * [0, n_rows) skips that token's k and v (padding); no two tokens may name the
+ * same slot.  Without slots, row t.
+ *   f_i = theta^(-2 i / rope_dim) / freq_factors[i] (1 where NULL), then
+ *   scaling 1 (linear): f_i / factor
+ *   scaling 2 (by parts): f_i (1 - r_i) + f_i / factor r_i, where r_i rises
+ *     linearly from 0 at pair floor(d(beta_fast)) to 1 at pair
+ *     ceil(d(beta_slow)), d(n) = rope_dim log(orig_ctx / (2 pi n)) / (2 log theta)
+ *     (the ends held within [0, rope_dim - 1]); cos and sin are multiplied by
+ *     mscale.
+ * Angles are reduced in double, so positions up to 2^31 - 1 keep fp32 accuracy.
+ * In place (x_out == x with equal strides) is allowed; any other overlap of an
+ * output row with an input or output row is refused.  Rows may have any
+ * alignment of the element type (16-byte aligned ones are faster). */
+#define INFERNO_ROPE_HALF 0        /* pairs (i, i + rope_dim / 2), as inferno_attention_step */
+#define INFERNO_ROPE_INTERLEAVED 1 /* pairs (2 i, 2 i + 1) */
+#define INFERNO_ROPE_SCALE_NONE 0
+#define INFERNO_ROPE_SCALE_LINEAR 1
+#define INFERNO_ROPE_SCALE_PARTS 2
+typedef struct InfernoRope {
+  int32_t struct_size;
+  int32_t type;
+  int32_t n_tokens, n_heads, n_kv_heads, head_dim;
+  int32_t rope_dim;              /* even, 2..min(head_dim, 512) */
+  int32_t layout;                /* INFERNO_ROPE_HALF / _INTERLEAVED */
+  int32_t scaling;               /* INFERNO_ROPE_SCALE_* */
+  int32_t inverse;               /* 1: rotate back (also the gradient of the rotation) */
+  int32_t orig_ctx;              /* scaling 2: positions of the unscaled context */
+  int32_t n_rows;                /* rows of k_out / v_out that slots may name */
+  float theta;                   /* > 1 */
+  float factor;                  /* scaling 1, 2: > 0 */
+  float beta_fast, beta_slow;    /* scaling 2: turns over orig_ctx; 0 = 32 and 1 */
+  float mscale;                  /* factor of cos and sin; 0 = 1, or 0.1 log(factor) + 1 for scaling 2 with factor > 1 */
+  const float* freq_factors;     /* [rope_dim / 2] or NULL (GGUF tensor rope_freqs.weight) */
+  const int32_t* positions;      /* [n_tokens] */
+  const int32_t* slots;          /* [n_tokens] or NULL */
+  const void *q, *k, *v;         /* v only with slots, or NULL */
+  void *q_out, *k_out, *v_out;
+  int64_t q_stride, k_stride, v_stride;               /* elements between token rows */
+  int64_t q_out_stride, k_out_stride, v_out_stride;
+} InfernoRope;
+int inferno_rope(const InfernoRope* r, void* stream);
+
+/* Attention of n_tokens new tokens of each of `batch` sequences.  Token t of
+ * sequence b sees prefix_len rows that all sequences share (prefix_k,
+ * prefix_v [prefix_len][n_kv_heads][head_dim]: read once for the batch) and
+ * rows 0 .. lens[b] - n_tokens + t of its own slice (k_cache + b * seq_stride):
+ * the last n_tokens of its lens[b] rows are those of the tokens themselves.
+ *   out = sum_j p_j v_j, p = softmax_j(scale q . k_j) over both parts
+ * Query head h reads KV head h / (n_heads / n_kv_heads); no RoPE, norm or gate
+ * is applied.  A token that sees no row gets zeros.  lens are clamped to
+ * [0, max_len]; rows from lens[b] on are not read as values, whatever they
+ * hold.  Non-finite values in rows that are seen give non-finite outputs.
+ * scores (optional, fp32): scores[(b * n_kv_heads + h) * score_stride + j]
+ * gains the weight that own row j got, summed over the tokens and query heads
+ * of KV head h; entries from lens[b] on are left as they are.
+ * q and out [batch * n_tokens][n_heads][head_dim] with q_stride / out_stride
+ * elements between token rows; out may be q, and overlaps nothing else.
+ * head_dim 64, 128 or 256; pointers and strides multiples of 16 bytes (lens and
+ * scores: of 4).  Results do not depend on timing (no atomics). */
+typedef struct InfernoAttention {
+  int32_t struct_size;
+  int32_t type;
+  int32_t batch, n_tokens, n_heads, n_kv_heads, head_dim;
+  int32_t prefix_len;            /* 0: no shared part */
+  int32_t max_len;               /* rows of a slice that may be read; 0: no own part */
+  float scale;                   /* 0 = 1 / sqrt(head_dim) */
+  int64_t q_stride, out_stride, seq_stride, score_stride;
+  const void* q;
+  const void *prefix_k, *prefix_v;
+  const void *k_cache, *v_cache;
+  const int32_t* lens;           /* [batch] */
+  float* scores;                 /* or NULL */
+  void* out;
+} InfernoAttention;
+/* bytes of workspace for a call with these sizes (a 256-byte aligned device
+ * buffer), or a negative status; reads no pointer but whether scores is set */
+int64_t inferno_attention_cached_workspace(const InfernoAttention* a);
+int inferno_attention_cached(const InfernoAttention* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Eviction: cuts each (sequence, KV head) with lens[b] > budget to budget
+ * rows.  Kept are, in this order: rows whose position slot_pos is < n_sink or
+ * >= next_pos[b] - n_recent, then rows by falling scores; ties go to the lower
+ * row, NaN ranks below everything.  (Should the first kind exceed the budget,
+ * they are ranked by score too.)  Kept rows at or behind `budget` move into the
+ * holes before it, both in rising order, with their K, V, score and position;
+ * nothing else moves, so the order of rows is not that of positions.  Each KV
+ * head chooses its own rows.  lens_out[b] = min(lens[b], budget); scores_out
+ * and slot_pos_out receive the rows 0 .. lens_out[b] - 1; rows behind are left
+ * as they were, in the caches too.  Sequences within the budget are copied
+ * through.  Layouts: caches as in inferno_attention_cached, scores and slot_pos
+ * [batch][n_kv_heads] rows of score_stride entries; outputs may be the inputs
+ * (same pointer) and overlap nothing else.  lens are clamped to [0, max_len]. */
+typedef struct InfernoEvict {
+  int32_t struct_size;
+  int32_t type;
+  int32_t batch, n_kv_heads, head_dim;
+  int32_t max_len;
+  int32_t budget;                /* >= 1 */
+  int32_t n_sink, n_recent;      /* n_sink + n_recent <= budget */
+  int32_t reserved;              /* 0 */
+  int64_t seq_stride, score_stride;
+  void *k_cache, *v_cache;
+  const float* scores;
+  const int32_t* slot_pos;
+  const int32_t* lens;           /* [batch] */
+  const int32_t* next_pos;       /* [batch]: position of the next token */
+  float* scores_out;
+  int32_t* slot_pos_out;
+  int32_t* lens_out;
+} InfernoEvict;
+int64_t inferno_cache_evict_workspace(const InfernoEvict* e);
+int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Sampling parameters of generate_cpu / softmax_sample
  * (src/ModelCPU.jl:1123-1225): temperature 0 = greedy. */

@@ -1,0 +1,771 @@
+// Attention of a few new tokens per sequence over a shared prefix and the
+// sequence's own cache (inferno_attention_cached).
+//
+//   out = sum_j p_j v_j,  p = softmax_j(scale q . k_j) over prefix and own rows
+//
+// Bound: the bytes of K and V, read once, while a KV head has few query rows
+// (n_tokens x group for its own rows, batch x n_tokens x group for the prefix).
+//
+// ac_part_kernel: a CTA takes 16 R query rows of one KV head (prefix: of all
+// sequences; own part: of one) against one split of the keys.  Its warps form NG
+// key groups of R warps; each group walks its own tiles of 16 keys with a ring of
+// cp.async slots (a K or a V tile per slot, rows past the end zero-filled), each
+// warp holds 16 rows: S = Q K^T and O += P V by mma.sync with the running
+// maximum and sum of the softmax in registers.  mma.sync because a tile of
+// 16 rows cannot fill the 128-row tcgen05 instruction and the kernel is bound by
+// bytes; fp32 operands are carried as tf32 pairs (hi, lo) in three products,
+// about 21 significant bits.  The groups merge in shared memory.
+// ac_finish_kernel: joins the splits of a row, and adds the weights of the own
+// rows to `scores` from the logits that the first kernel left.
+#include <algorithm>
+#include <cmath>
+#include <cuda_bf16.h>
+#include "internal.h"
+#include "common.cuh"
+#include "attn_cached.h"
+#include "longctx.h"
+#include "../../include/inferno_b200.h"
+
+namespace inf {
+
+namespace {
+
+constexpr int AC_KT = 16;                       // keys per tile
+constexpr int AC_SMEM = 227 * 1024;
+constexpr int AC_FIN_THREADS = 256;
+constexpr int AC_FIN_SLOTS = AC_FIN_THREADS;    // own rows per finishing CTA
+
+template <typename T>
+struct AcType;
+template <>
+struct AcType<float> { static constexpr bool F32 = true; };
+template <>
+struct AcType<__half> { static constexpr bool F32 = false; };
+template <>
+struct AcType<__nv_bfloat16> { static constexpr bool F32 = false; };
+
+// geometry of one instantiation
+template <typename T, int HD, int R>
+struct AcGeo {
+  static constexpr int ROW = HD * (int)sizeof(T);              // bytes of a K / V row of one head
+  static constexpr int ITEM = AC_KT * ROW;                     // bytes of a ring slot
+  static constexpr int QBYTES = AcType<T>::F32 ? 16 * R * ROW : 0;
+  // eight warps (512 threads could not hold the accumulators of head_dim 256);
+  // fewer groups where three slots each would not fit
+  static constexpr int NG0 = 8 / R;
+  static constexpr int ROOM = AC_SMEM - 1024 - QBYTES;
+  static constexpr int NG = NG0 * 3 * ITEM <= ROOM ? NG0 : NG0 / 2;
+  static constexpr int NW = NG * R;
+  static constexpr int THREADS = NW * 32;
+  static constexpr int MAXSLOTS = ROOM / (NG * ITEM);
+  static constexpr int SLOTS = MAXSLOTS > 6 ? 6 : MAXSLOTS;
+  static constexpr int RING = NG * SLOTS * ITEM;
+  static constexpr int MERGE = NW * 16 * HD * 4;
+  static constexpr int SMEM = QBYTES + (RING > MERGE ? RING : MERGE) + NW * 16 * 8;
+  static_assert(SLOTS >= 3 && SMEM <= AC_SMEM, "shared memory");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm_x4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo: hi rounded to tf32's 11 significant bits (half up in magnitude),
+// lo the exact rest, of which the instruction reads the leading 11 bits
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&h;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&h;
+  }
+}
+
+// address of the 16-byte chunk c of row r of a tile; the exclusive-or spreads the
+// rows that one access touches over all banks
+template <int ROW>
+__device__ __forceinline__ uint32_t tile_addr(uint32_t base, int r, int c) {
+  return base + r * ROW + ((c ^ (r & 7)) << 4);
+}
+
+// what a CTA works on
+struct AcWork {
+  const uint8_t *k, *v;      // first key row of the KV head
+  int j0, j1;                // keys
+  int row0, nrows;           // rows of this CTA among its part's; their number
+  int b;                     // own part: the sequence (prefix: -1)
+  int kvh, split;            // split index among n_splits
+  int len;                   // own part: lens[b]
+};
+
+// row `r` of a part (prefix: over all sequences) -> (b, t, h)
+__device__ __forceinline__ void ac_row(const AcParams& p, const AcWork& w, int r, int& b, int& t, int& h) {
+  const int per_b = p.n_tok * p.group;
+  b = w.b;
+  if (b < 0) {
+    b = r / per_b;
+    r -= b * per_b;
+  }
+  t = r / p.group;
+  h = w.kvh * p.group + (r - t * p.group);
+}
+
+// factor of a part with statistics (largest logit, sum) in a row whose largest
+// logit is M.  A part without keys has weight 0; one whose logits are all NaN
+// also has no largest logit, but its sum is NaN, and so is its weight here.
+__device__ __forceinline__ float ac_weight(float2 ml, float M) {
+  return ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - M);
+}
+
+template <typename T, int HD, int R>
+__global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(const __grid_constant__ AcParams p, int prefix_part, int row_tiles) {
+  using G = AcGeo<T, HD, R>;
+  constexpr bool F32 = AcType<T>::F32;
+  constexpr int ROW = G::ROW, ITEM = G::ITEM, SLOTS = G::SLOTS, GT = R * 32;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const int grp = warp / R, rt = warp - grp * R;       // key group, row tile of the warp
+  const int gtid = tid - grp * GT;                     // thread within the group
+
+  AcWork w;
+  {
+    int x = blockIdx.x;
+    const int splits = prefix_part ? p.p_splits : p.o_splits;
+    w.split = x % splits;
+    x /= splits;
+    w.row0 = (x % row_tiles) * 16 * R;
+    x /= row_tiles;
+    w.kvh = x % p.nkv;
+    x /= p.nkv;
+    const int rows = p.n_tok * p.group;
+    if (prefix_part) {
+      w.b = -1;
+      w.nrows = p.batch * rows;
+      w.len = p.prefix_len;
+      w.j0 = w.split * p.p_split_len;
+      w.j1 = min(w.len, w.j0 + p.p_split_len);
+      w.k = (const uint8_t*)p.pk;
+      w.v = (const uint8_t*)p.pv;
+    } else {
+      w.b = x;
+      w.nrows = rows;
+      w.len = max(0, min(p.lens[x], p.max_len));
+      w.j0 = w.split * p.o_split_len;
+      w.j1 = min(w.len, w.j0 + p.o_split_len);
+      w.k = (const uint8_t*)p.kc + (long long)x * p.seq_stride * (int)sizeof(T);
+      w.v = (const uint8_t*)p.vc + (long long)x * p.seq_stride * (int)sizeof(T);
+      w.split += p.p_splits;
+    }
+    w.k += (long long)w.kvh * ROW;
+    w.v += (long long)w.kvh * ROW;
+  }
+  if (w.j0 >= w.j1) return;          // nothing of this sequence in this split
+  const long long key_stride = (long long)p.nkv * ROW;
+
+  const uint32_t s_q = smem_u32(smem);                            // fp32 only: [16 R][HD]
+  uint8_t* ring_p = smem + G::QBYTES;
+  const uint32_t ring = smem_u32(ring_p) + grp * SLOTS * ITEM;
+  float2* s_ml = (float2*)(ring_p + (G::RING > G::MERGE ? G::RING : G::MERGE));   // [NW][16]
+
+  // tiles of this group: grp, grp + NG, ...; item 2 i is K of its i-th tile, 2 i + 1 V
+  const int ntiles = (w.j1 - w.j0 + AC_KT - 1) / AC_KT;
+  const int my_tiles = ntiles > grp ? (ntiles - grp + G::NG - 1) / G::NG : 0;
+  const int items = 2 * my_tiles;
+  auto issue = [&](int item) {
+    if (item < items) {
+      const int key0 = w.j0 + (grp + (item >> 1) * G::NG) * AC_KT;
+      const uint8_t* src = (item & 1) ? w.v : w.k;
+      const uint32_t dst = ring + (item % SLOTS) * ITEM;
+      constexpr int CH = ROW / 16;
+#pragma unroll
+      for (int i = 0; i < AC_KT * CH / GT; ++i) {
+        const int id = i * GT + gtid, r = id / CH, c = id % CH;
+        const bool ok = key0 + r < w.j1;
+        cp_async16(tile_addr<ROW>(dst, r, c), src + (ok ? (long long)(key0 + r) * key_stride : 0) + c * 16, ok);
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS - 1; ++i) issue(i);
+
+  // ---- Q: 16-bit types in registers as A fragments, fp32 in shared memory ----
+  uint32_t qf[F32 ? 1 : HD / 16][4];
+  const int r_lo = w.row0 + rt * 16 + g, r_hi = r_lo + 8;         // the two rows of this thread
+  int lim_lo = 0, lim_hi = 0;                                     // keys they see
+  {
+    int b, t, h;
+    const T *q_lo = nullptr, *q_hi = nullptr;
+    if (r_lo < w.nrows) {
+      ac_row(p, w, r_lo, b, t, h);
+      q_lo = (const T*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD;
+      lim_lo = w.b < 0 ? w.len : w.len - p.n_tok + 1 + t;
+    }
+    if (r_hi < w.nrows) {
+      ac_row(p, w, r_hi, b, t, h);
+      q_hi = (const T*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD;
+      lim_hi = w.b < 0 ? w.len : w.len - p.n_tok + 1 + t;
+    }
+    if constexpr (!F32) {
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        const int d = 16 * k + 2 * t4;
+        qf[k][0] = q_lo ? *(const uint32_t*)(q_lo + d) : 0u;
+        qf[k][1] = q_hi ? *(const uint32_t*)(q_hi + d) : 0u;
+        qf[k][2] = q_lo ? *(const uint32_t*)(q_lo + d + 8) : 0u;
+        qf[k][3] = q_hi ? *(const uint32_t*)(q_hi + d + 8) : 0u;
+      }
+    } else {
+      for (int id = tid; id < 16 * R * (ROW / 16); id += G::THREADS) {
+        const int r = id / (ROW / 16), c = id % (ROW / 16);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (w.row0 + r < w.nrows) {
+          ac_row(p, w, w.row0 + r, b, t, h);
+          x = *(const float4*)((const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD + 4 * c);
+        }
+        *(float4*)(smem + (tile_addr<ROW>(0, r, c))) = x;
+      }
+      __syncthreads();
+    }
+  }
+  float* lg_lo = nullptr;
+  float* lg_hi = nullptr;
+  if (p.scores && w.b >= 0) {
+    int b, t, h;
+    if (r_lo < w.nrows) {
+      ac_row(p, w, r_lo, b, t, h);
+      lg_lo = p.logits + ((long long)(b * p.n_tok + t) * p.nh + h) * p.logit_stride;
+    }
+    if (r_hi < w.nrows) {
+      ac_row(p, w, r_hi, b, t, h);
+      lg_hi = p.logits + ((long long)(b * p.n_tok + t) * p.nh + h) * p.logit_stride;
+    }
+  }
+
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+  float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
+
+  auto landed = [&]() {
+    cp_wait<SLOTS - 2>();
+    if constexpr (R == 1) __syncwarp();
+    else named_bar_sync(1 + grp, GT);
+  };
+
+  for (int i = 0; i < my_tiles; ++i) {
+    const int key0 = w.j0 + (grp + i * G::NG) * AC_KT;
+    // ---- S = Q K^T ----
+    landed();
+    issue(2 * i + SLOTS - 1);
+    const uint32_t kt = ring + ((2 * i) % SLOTS) * ITEM;
+    float s[2][4];
+    if constexpr (!F32) {
+      float c[2][2][4];              // even and odd k steps apart: shorter dependence chains
+#pragma unroll
+      for (int a = 0; a < 16; ++a) c[a >> 3][(a >> 2) & 1][a & 3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        uint32_t kb[4];
+        ldsm_x4(tile_addr<ROW>(kt, (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)), kb);
+        mma16<T>(c[k & 1][0], qf[k], kb[0], kb[1]);
+        mma16<T>(c[k & 1][1], qf[k], kb[2], kb[3]);
+      }
+#pragma unroll
+      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] = c[0][a >> 2][a & 3] + c[1][a >> 2][a & 3];
+    } else {
+      float c[2][3][4];              // per n tile: hi hi, hi lo, lo hi
+#pragma unroll
+      for (int a = 0; a < 24; ++a) c[a / 12][(a / 4) % 3][a & 3] = 0.f;
+#pragma unroll
+      for (int cg = 0; cg < HD / 32; ++cg)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // four consecutive dims per thread, used as the k indices t4 and t4 + 4
+          // of two k steps, the same dims of Q and K
+          const int ch = 8 * cg + 2 * t4 + e;
+          const float4 qa = lds_f4(tile_addr<ROW>(s_q, rt * 16 + g, ch));
+          const float4 qb = lds_f4(tile_addr<ROW>(s_q, rt * 16 + g + 8, ch));
+          const float4 k0 = lds_f4(tile_addr<ROW>(kt, g, ch));
+          const float4 k1 = lds_f4(tile_addr<ROW>(kt, g + 8, ch));
+          const float qv[2][4] = {{qa.x, qb.x, qa.y, qb.y}, {qa.z, qb.z, qa.w, qb.w}};
+          const float kv[2][2][2] = {{{k0.x, k0.y}, {k1.x, k1.y}}, {{k0.z, k0.w}, {k1.z, k1.w}}};
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            uint32_t ah[4], al[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) split_tf32(qv[st][x], ah[x], al[x]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              uint32_t h0, h1, l0, l1;
+              split_tf32(kv[st][n][0], h0, l0);
+              split_tf32(kv[st][n][1], h1, l1);
+              mma_tf32(c[n][0], ah, h0, h1);
+              mma_tf32(c[n][1], ah, l0, l1);
+              mma_tf32(c[n][2], al, h0, h1);
+            }
+          }
+        }
+#pragma unroll
+      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] = c[a >> 2][0][a & 3] + (c[a >> 2][1][a & 3] + c[a >> 2][2][a & 3]);
+    }
+    // ---- running softmax ----
+    float mx_lo = -INFINITY, mx_hi = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int key = key0 + 8 * n + 2 * t4 + x;
+        const bool in = key < w.j1;
+        s[n][x] = in && key < lim_lo ? s[n][x] * p.scale_log2 : -INFINITY;
+        s[n][2 + x] = in && key < lim_hi ? s[n][2 + x] * p.scale_log2 : -INFINITY;
+        mx_lo = fmaxf(mx_lo, s[n][x]);
+        mx_hi = fmaxf(mx_hi, s[n][2 + x]);
+      }
+#pragma unroll
+    for (int of = 1; of <= 2; of <<= 1) {
+      mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, of));
+      mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, of));
+    }
+    if (lg_lo) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) *(float2*)(lg_lo + key0 + 8 * n + 2 * t4) = make_float2(s[n][0], s[n][1]);
+    }
+    if (lg_hi) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) *(float2*)(lg_hi + key0 + 8 * n + 2 * t4) = make_float2(s[n][2], s[n][3]);
+    }
+    if (__any_sync(0xffffffffu, mx_lo > m_lo || mx_hi > m_hi)) {
+      const float n_lo = fmaxf(m_lo, mx_lo), n_hi = fmaxf(m_hi, mx_hi);
+      const float f_lo = n_lo == -INFINITY ? 1.f : exp2f(m_lo - n_lo), f_hi = n_hi == -INFINITY ? 1.f : exp2f(m_hi - n_hi);
+      m_lo = n_lo, m_hi = n_hi;
+      l_lo *= f_lo, l_hi *= f_hi;
+#pragma unroll
+      for (int x = 0; x < HD / 8; ++x) o[x][0] *= f_lo, o[x][1] *= f_lo, o[x][2] *= f_hi, o[x][3] *= f_hi;
+    }
+    const float z_lo = m_lo == -INFINITY ? 0.f : m_lo, z_hi = m_hi == -INFINITY ? 0.f : m_hi;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        s[n][x] = exp2f(s[n][x] - z_lo);
+        s[n][2 + x] = exp2f(s[n][2 + x] - z_hi);
+        l_lo += s[n][x];
+        l_hi += s[n][2 + x];
+      }
+    // ---- O += P V ----
+    landed();
+    issue(2 * i + 1 + SLOTS - 1);
+    const uint32_t vt = ring + ((2 * i + 1) % SLOTS) * ITEM;
+    if constexpr (!F32) {
+      // P rounded to the 16-bit type, as V is: half a step (2^-9, 2^-12) per
+      // term, below the rounding of the output
+      const uint32_t pa[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
+                              pack2<T>(s[1][2], s[1][3])};
+#pragma unroll
+      for (int n = 0; n < HD / 16; ++n) {
+        uint32_t vb[4];
+        ldsm_x4_t(tile_addr<ROW>(vt, ((lane >> 3) & 1) * 8 + (lane & 7), 2 * n + (lane >> 4)), vb);
+        mma16<T>(o[2 * n], pa, vb[0], vb[1]);
+        mma16<T>(o[2 * n + 1], pa, vb[2], vb[3]);
+      }
+    } else {
+      // the k index t4 of step n is key 8 n + 2 t4, t4 + 4 is key 8 n + 2 t4 + 1:
+      // the accumulator layout of S is the A layout of P
+      uint32_t ph[2][4], pl[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        split_tf32(s[n][0], ph[n][0], pl[n][0]);
+        split_tf32(s[n][2], ph[n][1], pl[n][1]);
+        split_tf32(s[n][1], ph[n][2], pl[n][2]);
+        split_tf32(s[n][3], ph[n][3], pl[n][3]);
+      }
+#pragma unroll
+      for (int cg = 0; cg < HD / 32; ++cg)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          // dims 32 cg + 4 g + x are column g of n tile 4 cg + x
+          const float4 v0 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4, 8 * cg + g));
+          const float4 v1 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4 + 1, 8 * cg + g));
+          const float a[4] = {v0.x, v0.y, v0.z, v0.w}, b[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t h0, h1, l0, l1;
+            split_tf32(a[x], h0, l0);
+            split_tf32(b[x], h1, l1);
+            mma_tf32(o[4 * cg + x], ph[n], h0, h1);
+            mma_tf32(o[4 * cg + x], ph[n], l0, l1);
+            mma_tf32(o[4 * cg + x], pl[n], h0, h1);
+          }
+        }
+    }
+  }
+
+  // ---- merge the key groups ----
+#pragma unroll
+  for (int of = 1; of <= 2; of <<= 1) {
+    l_lo += __shfl_xor_sync(0xffffffffu, l_lo, of);
+    l_hi += __shfl_xor_sync(0xffffffffu, l_hi, of);
+  }
+  if (t4 == 0) {
+    s_ml[warp * 16 + g] = make_float2(m_lo, l_lo);
+    s_ml[warp * 16 + g + 8] = make_float2(m_hi, l_hi);
+  }
+  cp_wait<0>();
+  __syncthreads();                     // every group is done with its ring
+  float M_lo = -INFINITY, M_hi = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < G::NG; ++x) {
+    M_lo = fmaxf(M_lo, s_ml[(x * R + rt) * 16 + g].x);
+    M_hi = fmaxf(M_hi, s_ml[(x * R + rt) * 16 + g + 8].x);
+  }
+  const float f_lo = ac_weight(make_float2(m_lo, l_lo), M_lo), f_hi = ac_weight(make_float2(m_hi, l_hi), M_hi);
+  float* mo = (float*)ring_p + (long long)warp * 16 * HD;      // [16][HD]
+  if constexpr (!F32) {
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n) {
+      *(float2*)(mo + g * HD + 8 * n + 2 * t4) = make_float2(o[n][0] * f_lo, o[n][1] * f_lo);
+      *(float2*)(mo + (g + 8) * HD + 8 * n + 2 * t4) = make_float2(o[n][2] * f_hi, o[n][3] * f_hi);
+    }
+  } else {
+#pragma unroll
+    for (int cg = 0; cg < HD / 32; ++cg)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int d = 32 * cg + 8 * t4 + 4 * x;
+        *(float4*)(mo + g * HD + d) = make_float4(o[4 * cg][x] * f_lo, o[4 * cg + 1][x] * f_lo, o[4 * cg + 2][x] * f_lo, o[4 * cg + 3][x] * f_lo);
+        *(float4*)(mo + (g + 8) * HD + d) = make_float4(o[4 * cg][2 + x] * f_hi, o[4 * cg + 1][2 + x] * f_hi, o[4 * cg + 2][2 + x] * f_hi, o[4 * cg + 3][2 + x] * f_hi);
+      }
+  }
+  __syncthreads();
+  const int live = min(16 * R, w.nrows - w.row0);
+  for (int id = tid; id < live * (HD / 4); id += G::THREADS) {
+    const int r = id / (HD / 4), c = id % (HD / 4), tile = r >> 4, rr = r & 15;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < G::NG; ++x) {
+      const float4 y = *(const float4*)((const float*)ring_p + ((long long)(x * R + tile) * 16 + rr) * HD + 4 * c);
+      a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
+    }
+    int b, t, h;
+    ac_row(p, w, w.row0 + r, b, t, h);
+    const long long at = ((long long)(b * p.n_tok + t) * p.nh + h) * p.n_splits + w.split;
+    *(float4*)(p.part_o + at * HD + 4 * c) = a;
+    if (c == 0) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int x = 0; x < G::NG; ++x) M = fmaxf(M, s_ml[(x * R + tile) * 16 + rr].x);
+#pragma unroll
+      for (int x = 0; x < G::NG; ++x) {
+        const float2 y = s_ml[(x * R + tile) * 16 + rr];
+        L += y.y * ac_weight(y, M);
+      }
+      p.part_ml[at] = make_float2(M, L);
+    }
+  }
+}
+
+// splits of a row that hold something: all of the prefix, own ones up to lens
+__device__ __forceinline__ int ac_live_splits(const AcParams& p, int b) {
+  int n = p.p_splits;
+  if (p.o_splits) {
+    const int len = max(0, min(p.lens[b], p.max_len));
+    n += (len + p.o_split_len - 1) / p.o_split_len;
+  }
+  return n;
+}
+// (largest logit, 1 / sum) over a row's splits; called by a whole warp
+__device__ __forceinline__ float2 ac_row_stats(const AcParams& p, long long row, int n) {
+  const float2* ml = p.part_ml + row * p.n_splits;
+  float M = -INFINITY;
+  for (int s = threadIdx.x & 31; s < n; s += 32) M = fmaxf(M, ml[s].x);
+  M = warp_max(M);
+  float L = 0.f;
+  for (int s = threadIdx.x & 31; s < n; s += 32) {
+    const float2 x = ml[s];
+    L += x.y * ac_weight(x, M);
+  }
+  L = warp_sum(L);
+  return make_float2(M, L > 0.f ? 1.f / L : (L == L ? 0.f : L));
+}
+
+// blocks [0, row_blocks): one warp per row joins its splits; blocks behind:
+// `scores` of one (sequence, KV head), AC_FIN_SLOTS own rows each
+template <typename T, int HD>
+__global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_constant__ AcParams p, int row_blocks, int slot_blocks) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x < row_blocks) {
+    const long long row = (long long)blockIdx.x * (AC_FIN_THREADS / 32) + warp;
+    const long long tok = row / p.nh;
+    const int h = (int)(row - tok * p.nh);
+    if (tok >= (long long)p.batch * p.n_tok) return;
+    const int n = ac_live_splits(p, (int)(tok / p.n_tok));
+    const float2 st = ac_row_stats(p, row, n);
+    constexpr int PER = HD / 32;                     // dims of a lane
+    float a[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) a[i] = 0.f;
+    for (int s = 0; s < n; ++s) {
+      const float f = ac_weight(p.part_ml[row * p.n_splits + s], st.x);
+      const float* o = p.part_o + (row * p.n_splits + s) * HD + lane * PER;
+#pragma unroll
+      for (int i = 0; i < PER; i += 2) {
+        const float2 x = *(const float2*)(o + i);
+        a[i] = fmaf(f, x.x, a[i]);
+        a[i + 1] = fmaf(f, x.y, a[i + 1]);
+      }
+    }
+    T* out = (T*)p.out + tok * p.out_stride + (long long)h * HD + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) {
+      const float x = a[i] * st.y, y = a[i + 1] * st.y;
+      if constexpr (AcType<T>::F32) *(float2*)(out + i) = make_float2(x, y);
+      else *(uint32_t*)(out + i) = pack2<T>(x, y);
+    }
+    return;
+  }
+  constexpr int CHUNK = 64;                          // rows whose statistics are held at once
+  __shared__ float2 st[CHUNK];
+  const int x = blockIdx.x - row_blocks, bh = x / slot_blocks, b = bh / p.nkv, kvh = bh - b * p.nkv;
+  const int j = (x - bh * slot_blocks) * AC_FIN_SLOTS + threadIdx.x;
+  const int len = max(0, min(p.lens[b], p.max_len));
+  if (j - (int)threadIdx.x >= len) return;
+  const int n = ac_live_splits(p, b), rows = p.n_tok * p.group;
+  float sum = 0.f;
+  for (int r0 = 0; r0 < rows; r0 += CHUNK) {
+    const int nr = min(CHUNK, rows - r0);
+    __syncthreads();
+    for (int r = warp; r < nr; r += AC_FIN_THREADS / 32) {
+      const int t = (r0 + r) / p.group, h = kvh * p.group + (r0 + r) - t * p.group;
+      const float2 s = ac_row_stats(p, (long long)(b * p.n_tok + t) * p.nh + h, n);
+      if (lane == 0) st[r] = s;
+    }
+    __syncthreads();
+    if (j < len)
+      for (int r = 0; r < nr; ++r) {
+        const int t = (r0 + r) / p.group, h = kvh * p.group + (r0 + r) - t * p.group;
+        const float lg = p.logits[((long long)(b * p.n_tok + t) * p.nh + h) * p.logit_stride + j];
+        if (lg != -INFINITY) sum += exp2f(lg - st[r].x) * st[r].y;
+      }
+  }
+  if (j < len) p.scores[(long long)bh * p.score_stride + j] += sum;
+}
+
+// ---- host ---------------------------------------------------------------------
+struct AcPlan {
+  int p_r, o_r;                   // 16-row tiles per CTA of the two parts
+  int p_tiles, o_tiles;           // row tiles
+  long long rows;                 // query rows over all heads
+  size_t off_ml, off_logits, bytes;
+};
+
+int ac_row_class(long long rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+// Splits of `len` keys for `units` CTAs' worth of other work: enough CTAs for
+// `waves` per SM, but at least 128 keys (eight tiles of 16) each, and at most 256
+void ac_split(long long units, int len, int waves, int* splits, int* split_len) {
+  if (len <= 0) {
+    *splits = 0;
+    *split_len = 16;
+    return;
+  }
+  long long want = std::max(1ll, (148ll * waves + units - 1) / units);
+  want = std::min(want, 256ll);
+  int sl = (int)((len + want - 1) / want);
+  sl = std::max(128, (sl + 127) / 128 * 128);
+  *split_len = sl;
+  *splits = (len + sl - 1) / sl;
+}
+
+int ac_check(const InfernoAttention* a) {
+  if (!a) return set_error(INFERNO_EINVAL, "attention_cached: null parameters");
+  if (a->struct_size != (int)sizeof(InfernoAttention))
+    return set_error(INFERNO_EINVAL, "attention_cached: struct_size %d, expected %d", a->struct_size,
+                     (int)sizeof(InfernoAttention));
+  if (!longctx_type_size(a->type))
+    return set_error(INFERNO_EINVAL, "attention_cached: type %d is not F32, F16 or BF16", a->type);
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+    return set_error(INFERNO_EINVAL, "attention_cached: head_dim %d is not 64, 128 or 256", a->head_dim);
+  if (a->batch < 0 || a->n_tokens < 1 || a->n_heads < 1 || a->n_kv_heads < 1 || a->n_heads % a->n_kv_heads)
+    return set_error(INFERNO_EINVAL, "attention_cached: bad sizes (batch %d, %d tokens, %d / %d heads)", a->batch,
+                     a->n_tokens, a->n_heads, a->n_kv_heads);
+  if (a->prefix_len < 0 || a->max_len < 0)
+    return set_error(INFERNO_EINVAL, "attention_cached: prefix_len %d, max_len %d", a->prefix_len, a->max_len);
+  if (a->prefix_len > (1 << 30) || a->max_len > (1 << 30) || a->n_heads > 65536 ||
+      (double)a->batch * a->n_tokens * a->n_heads > (double)(1 << 24))
+    return set_error(INFERNO_EINVAL, "attention_cached: more than 2^24 query rows or 2^30 keys");
+  if (!std::isfinite(a->scale)) return set_error(INFERNO_EINVAL, "attention_cached: scale is not finite");
+  return 0;
+}
+
+AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
+  AcPlan pl{};
+  p->batch = a->batch;
+  p->n_tok = a->n_tokens;
+  p->nh = a->n_heads;
+  p->nkv = a->n_kv_heads;
+  p->group = a->n_heads / a->n_kv_heads;
+  p->prefix_len = a->prefix_len;
+  p->max_len = a->max_len;
+  const long long own = (long long)a->n_tokens * p->group, pre = own * a->batch;
+  pl.rows = pre * a->n_kv_heads;
+  pl.o_r = ac_row_class(own);
+  pl.p_r = ac_row_class(pre);
+  pl.o_tiles = (int)((own + 16 * pl.o_r - 1) / (16 * pl.o_r));
+  pl.p_tiles = (int)((pre + 16 * pl.p_r - 1) / (16 * pl.p_r));
+  ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, 1, &p->p_splits, &p->p_split_len);
+  ac_split((long long)pl.o_tiles * a->n_kv_heads * a->batch, a->max_len, 2, &p->o_splits, &p->o_split_len);
+  p->n_splits = p->p_splits + p->o_splits;
+  p->logit_stride = a->scores ? ((long long)a->max_len + 15) / 16 * 16 : 0;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  pl.off_ml = up((size_t)pl.rows * p->n_splits * a->head_dim * 4);
+  pl.off_logits = pl.off_ml + up((size_t)pl.rows * p->n_splits * 8);
+  pl.bytes = pl.off_logits + up((size_t)pl.rows * p->logit_stride * 4) + 256;
+  return pl;
+}
+
+template <typename T, int HD, int R>
+cudaError_t ac_launch_part(const AcParams& p, int prefix_part, int tiles, long long blocks, cudaStream_t st) {
+  using G = AcGeo<T, HD, R>;
+  static DeviceOnce once;
+  cudaError_t e = once.run([] {
+    return cudaFuncSetAttribute(ac_part_kernel<T, HD, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+  });
+  if (e != cudaSuccess) return e;
+  ac_part_kernel<T, HD, R><<<(unsigned)blocks, G::THREADS, G::SMEM, st>>>(p, prefix_part, tiles);
+  return cudaGetLastError();
+}
+template <typename T, int HD>
+cudaError_t ac_part(const AcParams& p, int r, int prefix_part, int tiles, cudaStream_t st) {
+  const long long blocks = (long long)tiles * p.nkv * (prefix_part ? p.p_splits : (long long)p.o_splits * p.batch);
+  if (blocks <= 0) return cudaSuccess;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  return r == 1   ? ac_launch_part<T, HD, 1>(p, prefix_part, tiles, blocks, st)
+         : r == 2 ? ac_launch_part<T, HD, 2>(p, prefix_part, tiles, blocks, st)
+                  : ac_launch_part<T, HD, 4>(p, prefix_part, tiles, blocks, st);
+}
+template <typename T, int HD>
+cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
+  cudaError_t e = ac_part<T, HD>(p, pl.p_r, 1, pl.p_tiles, st);
+  if (e == cudaSuccess) e = ac_part<T, HD>(p, pl.o_r, 0, pl.o_tiles, st);
+  if (e != cudaSuccess) return e;
+  const long long row_blocks = (pl.rows + AC_FIN_THREADS / 32 - 1) / (AC_FIN_THREADS / 32);
+  const long long slot_blocks = p.scores ? (p.max_len + AC_FIN_SLOTS - 1) / AC_FIN_SLOTS : 0;
+  const long long blocks = row_blocks + slot_blocks * p.batch * p.nkv;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  ac_finish_kernel<T, HD><<<(unsigned)blocks, AC_FIN_THREADS, 0, st>>>(p, (int)row_blocks, (int)std::max(1ll, slot_blocks));
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t ac_run_hd(int hd, const AcParams& p, const AcPlan& pl, cudaStream_t st) {
+  return hd == 64 ? ac_run<T, 64>(p, pl, st) : hd == 128 ? ac_run<T, 128>(p, pl, st) : ac_run<T, 256>(p, pl, st);
+}
+
+}  // namespace
+}  // namespace inf
+
+using namespace inf;
+
+extern "C" int64_t inferno_attention_cached_workspace(const InfernoAttention* a) {
+  const int rc = ac_check(a);
+  if (rc) return rc;
+  AcParams p{};
+  return (int64_t)ac_plan(a, &p).bytes;
+}
+
+extern "C" int inferno_attention_cached(const InfernoAttention* a, void* workspace, int64_t workspace_bytes,
+                                        void* stream) {
+  int rc = ac_check(a);
+  if (rc) return rc;
+  if (a->batch == 0) return 0;
+  const long long es = longctx_type_size(a->type), row = (long long)a->n_kv_heads * a->head_dim;
+  const long long qrow = (long long)a->n_heads * a->head_dim;
+  if (!a->q || !a->out) return set_error(INFERNO_EINVAL, "attention_cached: q or out missing");
+  if (a->prefix_len && (!a->prefix_k || !a->prefix_v))
+    return set_error(INFERNO_EINVAL, "attention_cached: prefix_k or prefix_v missing");
+  if (a->max_len && (!a->k_cache || !a->v_cache || !a->lens))
+    return set_error(INFERNO_EINVAL, "attention_cached: k_cache, v_cache or lens missing");
+  if ((long long)a->batch * a->n_tokens > 1 && (a->q_stride < qrow || a->out_stride < qrow))
+    return set_error(INFERNO_EINVAL, "attention_cached: q_stride %lld or out_stride %lld is less than a token row of %lld",
+                     (long long)a->q_stride, (long long)a->out_stride, qrow);
+  if (a->max_len && a->batch > 1 && a->seq_stride < row * a->max_len)
+    return set_error(INFERNO_EINVAL, "attention_cached: seq_stride %lld is less than a slice of %d rows",
+                     (long long)a->seq_stride, a->max_len);
+  if (a->scores && (long long)a->batch * a->n_kv_heads > 1 && a->score_stride < a->max_len)
+    return set_error(INFERNO_EINVAL, "attention_cached: score_stride %lld is less than max_len %d",
+                     (long long)a->score_stride, a->max_len);
+  uintptr_t al = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)(a->q_stride * es) | (uintptr_t)(a->out_stride * es);
+  if (a->prefix_len) al |= (uintptr_t)a->prefix_k | (uintptr_t)a->prefix_v;
+  if (a->max_len) al |= (uintptr_t)a->k_cache | (uintptr_t)a->v_cache | (uintptr_t)(a->seq_stride * es);
+  if (al % 16) return set_error(INFERNO_EINVAL, "attention_cached: a pointer or stride is not a multiple of 16 bytes");
+  if (((uintptr_t)a->lens | (uintptr_t)a->scores) % 4)
+    return set_error(INFERNO_EINVAL, "attention_cached: lens or scores is not a multiple of 4 bytes");
+  AcParams p{};
+  const AcPlan pl = ac_plan(a, &p);
+  if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (int64_t)pl.bytes)
+    return set_error(INFERNO_EINVAL, "attention_cached: workspace of %lld bytes, %lld needed (256-byte aligned)",
+                     (long long)workspace_bytes, (long long)pl.bytes);
+  if ((rc = longctx_check_device(a->out, "attention_cached"))) return rc;
+  p.q = a->q;
+  p.pk = a->prefix_k;
+  p.pv = a->prefix_v;
+  p.kc = a->k_cache;
+  p.vc = a->v_cache;
+  p.lens = a->lens;
+  p.out = a->out;
+  p.scores = a->max_len ? a->scores : nullptr;
+  p.q_stride = a->q_stride;
+  p.out_stride = a->out_stride;
+  p.seq_stride = a->batch > 1 ? a->seq_stride : 0;
+  p.score_stride = a->score_stride;
+  p.scale_log2 = (a->scale == 0.0f ? 1.0f / sqrtf((float)a->head_dim) : a->scale) * AC_LOG2E;
+  p.part_o = (float*)workspace;
+  p.part_ml = (float2*)((char*)workspace + pl.off_ml);
+  p.logits = (float*)((char*)workspace + pl.off_logits);
+  cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = a->type == INFERNO_F32   ? ac_run_hd<float>(a->head_dim, p, pl, st)
+                        : a->type == INFERNO_F16 ? ac_run_hd<__half>(a->head_dim, p, pl, st)
+                                                 : ac_run_hd<__nv_bfloat16>(a->head_dim, p, pl, st);
+  return e == cudaSuccess ? 0 : set_error(INFERNO_ECUDA, "attention_cached launch: %s", cudaGetErrorString(e));
+}

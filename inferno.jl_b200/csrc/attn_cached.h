@@ -1,0 +1,33 @@
+// Shared declarations of the attention over a shared prefix and per-sequence
+// caches (attn_cached.cu, attn_prefix_tc.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace inf {
+
+// Query rows are numbered r = (b * n_tokens + t) * n_heads + h.  Every split of
+// the keys leaves, per row, its largest logit and the sum and weighted V sum of
+// exp2(logit - largest); logits are in units of log2.
+struct AcParams {
+  const void* q;
+  const void *pk, *pv;           // shared prefix [prefix_len][nkv][hd]
+  const void *kc, *vc;           // own slices [max_len][nkv][hd], seq_stride apart
+  const int* lens;
+  void* out;
+  float* scores;
+  long long q_stride, out_stride, seq_stride, score_stride;   // elements
+  int batch, n_tok, nh, nkv, group, prefix_len, max_len;
+  float scale_log2;              // scale * log2(e)
+  // splits: prefix splits come first, then own ones; split s of a part covers
+  // its keys [s * len, (s + 1) * len)
+  int p_splits, p_split_len, o_splits, o_split_len, n_splits;
+  float* part_o;                 // [row][n_splits][hd]
+  float2* part_ml;               // [row][n_splits] (largest logit, sum)
+  float* logits;                 // [row][logit_stride] own logits (only with scores)
+  long long logit_stride;
+};
+
+constexpr float AC_LOG2E = 1.4426950408889634f;
+
+}  // namespace inf

@@ -38,6 +38,41 @@ class InfernoSampling(C.Structure):
                 ("repetition_penalty", C.c_float), ("presence_penalty", C.c_float), ("seed", C.c_uint64)]
 
 
+class _Sized(C.Structure):
+    """A parameter struct whose struct_size is filled in."""
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(self)
+
+
+def _fields(kind, names):
+    return [(n, kind) for n in names.split()]
+
+
+class InfernoRope(_Sized):
+    """include/inferno_b200.h InfernoRope (rotary positions with cache append)."""
+    _fields_ = (_fields(C.c_int32, "struct_size type n_tokens n_heads n_kv_heads head_dim rope_dim layout scaling "
+                                   "inverse orig_ctx n_rows")
+                + _fields(C.c_float, "theta factor beta_fast beta_slow mscale")
+                + _fields(C.c_void_p, "freq_factors positions slots q k v q_out k_out v_out")
+                + _fields(C.c_int64, "q_stride k_stride v_stride q_out_stride k_out_stride v_out_stride"))
+
+
+class InfernoAttention(_Sized):
+    """include/inferno_b200.h InfernoAttention (shared prefix + per-sequence caches)."""
+    _fields_ = (_fields(C.c_int32, "struct_size type batch n_tokens n_heads n_kv_heads head_dim prefix_len max_len")
+                + _fields(C.c_float, "scale") + _fields(C.c_int64, "q_stride out_stride seq_stride score_stride")
+                + _fields(C.c_void_p, "q prefix_k prefix_v k_cache v_cache lens scores out"))
+
+
+class InfernoEvict(_Sized):
+    """include/inferno_b200.h InfernoEvict (cache eviction by gathered weight)."""
+    _fields_ = (_fields(C.c_int32, "struct_size type batch n_kv_heads head_dim max_len budget n_sink n_recent reserved")
+                + _fields(C.c_int64, "seq_stride score_stride")
+                + _fields(C.c_void_p, "k_cache v_cache scores slot_pos lens next_pos scores_out slot_pos_out lens_out"))
+
+
 # every symbol the header declares (checked by the CPU tests)
 EXPORTS = [
     "inferno_last_error", "inferno_version", "inferno_device_error",
@@ -54,6 +89,8 @@ EXPORTS = [
     "inferno_gguf_open", "inferno_gguf_close", "inferno_gguf_version", "inferno_gguf_n_tensors", "inferno_gguf_n_kv",
     "inferno_gguf_data_offset", "inferno_gguf_key", "inferno_gguf_tensor_info", "inferno_gguf_get_int",
     "inferno_gguf_get_float", "inferno_gguf_get_string", "inferno_gguf_get_array", "inferno_engine_load_gguf",
+    "inferno_rope", "inferno_attention_cached_workspace", "inferno_attention_cached", "inferno_cache_evict_workspace",
+    "inferno_cache_evict",
 ]
 
 _lib = None
@@ -129,6 +166,11 @@ def _sig(L0):
     L.inferno_gguf_get_array.argtypes = [p, C.c_char_p, p, p, p]
     L.inferno_engine_load_gguf.argtypes = [p, p]
     L.inferno_debug_xch_timeout.argtypes = [i, p]
+    L.inferno_rope.argtypes = [p, p]
+    for nm in ("inferno_attention_cached", "inferno_cache_evict"):
+        getattr(L, nm).argtypes = [p, p, i64, p]
+        getattr(L, nm + "_workspace").argtypes = [p]
+        getattr(L, nm + "_workspace").restype = i64
     L.inferno_attention_step.argtypes = [p, p, p, p, p, f, i, i, i, i, f, p, p, i, i, i, p, p]
 
 
