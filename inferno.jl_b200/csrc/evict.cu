@@ -1,15 +1,22 @@
 // Eviction of cache rows by gathered attention weight (inferno_cache_evict).
 //
-// Kernel 1, one CTA per (sequence, KV head): ranks the rows and decides which
-// stay.  The rank key is the score as an order-preserving 32-bit integer, in two
-// classes (rows kept always come first), and the budget-th largest key is found
-// by a radix select of four 8-bit digits; ties at that key go to the lowest rows.
-// One pass in row order then numbers the holes (evicted rows before the budget)
-// and the kept rows behind it; the i-th of these goes into the i-th hole, so the
-// two lists have equal lengths and no row is both read and written.  Scores and
-// positions are placed here.
-// Kernel 2 moves the K and V rows by the two lists.
+// One thread-block cluster per (sequence, KV head); each CTA owns a consecutive
+// part of the rows.  The rank key is the score as an order-preserving 32-bit
+// integer, in two classes (rows kept always come first); it is read once into
+// shared memory.  The budget-th largest key is found by a radix select of four
+// 8-bit digits: every CTA counts its own rows, reads the others' counts through
+// distributed shared memory and finds the digit for itself.  (Digits of 11 bits
+// save a barrier and cost eight times the remote reads, which are what a pass
+// waits for: 10 us a pass measured with 8 CTAs, 1 us with 8 bits.)
+// Ties at that key go to the lowest rows.  Which rows stay is then a bitmap, so
+// ranks are bit counts: the i-th kept row behind the budget goes into the i-th
+// hole before it.  The two lists have equal lengths and no row is both read and
+// written, so the CTAs of the cluster move K and V in any order.
+//
+// Bound: the bytes of the rows that move (read and written), after a chain of
+// six cluster barriers that few rows cannot hide.
 #include <algorithm>
+#include <cooperative_groups.h>
 #include "internal.h"
 #include "common.cuh"
 #include "longctx.h"
@@ -17,8 +24,14 @@
 
 namespace inf {
 
-constexpr int EV_THREADS = 1024;
-constexpr int EV_MOVE_THREADS = 256;
+namespace cg = cooperative_groups;
+
+constexpr int EV_THREADS = 512;
+constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_BINS = 256;
+constexpr int EV_MAX_CLUSTER = 8;
+constexpr int EV_MAX_LEN = 1 << 21;         // the bitmaps of a CTA's part fit shared memory up to here
+constexpr int EV_SMEM = 200 * 1024;
 
 struct EvictParams {
   uint8_t *kc, *vc;
@@ -28,154 +41,296 @@ struct EvictParams {
   const int* pos;
   const int *lens, *next_pos;
   float* scores_out;
-  int *pos_out, *lens_out;
+  int *pos_out, *lens_out;            // lens_out null: written by evict_lens_kernel
   long long stride;                   // entries between (sequence, KV head) rows of scores / pos
-  int batch, nkv, max_len, budget, n_sink, n_recent, max_moves;
-  int* counts;                        // [batch * nkv] rows to move
+  int nkv, max_len, budget, n_sink, n_recent, max_moves;
+  int words;                          // 32-row words a CTA's part may have
+  int cached;                         // keys held in shared memory
   int* lists;                         // [batch * nkv][2][max_moves]: holes, sources
 };
 
 // larger is kept first; NaN below everything; -0 equal to 0
 __device__ __forceinline__ uint32_t ev_key(float s) { return s != s ? 0u : float_ordered(s + 0.0f); }
 
-__device__ __forceinline__ bool ev_always(const EvictParams& p, int pos, int recent_from) {
-  return pos < p.n_sink || pos >= recent_from;
-}
+// what a CTA's peers read
+struct EvShared {
+  int hist[2][EV_BINS];               // counts of a digit
+  int4 border;                        // ties before / behind the budget, other rows to leave before it / to keep behind it
+  int always;                         // rows kept always
+  // the CTA's own
+  int total[EV_BINS];                 // counts over the cluster
+  int warp_sums[2][EV_WARPS];
+};
 
-// exclusive sums of v over the CTA in thread order; total in *sum
-__device__ __forceinline__ int2 ev_scan(int2 v, int2* warp_sums, int2* sum) {
+// exclusive sums of x and y over the CTA in thread order; the CTA's in sum_x, sum_y
+__device__ __forceinline__ void ev_scan(EvShared& s, int& x, int& y, int& sum_x, int& sum_y) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int2 x = v;
+  int a = x, b = y;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, x.x, o), b = __shfl_up_sync(0xffffffffu, x.y, o);
-    if (lane >= o) x.x += a, x.y += b;
+    const int u = __shfl_up_sync(0xffffffffu, a, o), v = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += u, b += v;
   }
   __syncthreads();
-  if (lane == 31) warp_sums[warp] = x;
+  if (lane == 31) s.warp_sums[0][warp] = a, s.warp_sums[1][warp] = b;
   __syncthreads();
-  int2 before = make_int2(0, 0), all = make_int2(0, 0);
-  for (int w = 0; w < EV_THREADS / 32; ++w) {
-    const int2 s = warp_sums[w];
-    if (w < warp) before.x += s.x, before.y += s.y;
-    all.x += s.x, all.y += s.y;
+  int ba = 0, bb = 0;
+  sum_x = sum_y = 0;
+#pragma unroll
+  for (int w = 0; w < EV_WARPS; ++w) {
+    const int u = s.warp_sums[0][w], v = s.warp_sums[1][w];
+    if (w < warp) ba += u, bb += v;
+    sum_x += u, sum_y += v;
   }
-  *sum = all;
-  return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+  x = ba + a - x;
+  y = bb + b - y;
 }
 
-__global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictParams p) {
-  const int bh = blockIdx.x, b = bh / p.nkv, t = threadIdx.x;
+__global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_constant__ EvictParams p) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int nc = cluster.num_blocks(), c = cluster.block_rank();
+  const int bh = blockIdx.x / nc, b = bh / p.nkv, h = bh - b * p.nkv;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  __shared__ EvShared sh;
+  extern __shared__ uint32_t ev_dyn[];
+  uint32_t* always = ev_dyn;                  // bit per row of the part: kept always
+  uint32_t* tie = always + p.words;           // key equal to the border
+  uint32_t* keep = tie + p.words;
+  int* base_h = (int*)(keep + p.words);       // holes / sources before a word
+  int* base_s = base_h + p.words;
+  uint32_t* skey = (uint32_t*)(base_s + p.words);
+
   const int len = max(0, min(p.lens[b], p.max_len));
+  if (p.lens_out && h == 0 && c == 0 && t == 0) p.lens_out[b] = min(len, p.budget);
   const float* sc = p.scores + bh * p.stride;
   const int* ps = p.pos + bh * p.stride;
   float* so = p.scores_out + bh * p.stride;
   int* po = p.pos_out + bh * p.stride;
-  if (len <= p.budget) {
-    if (so != sc)
-      for (int j = t; j < len; j += EV_THREADS) so[j] = sc[j];
-    if (po != ps)
-      for (int j = t; j < len; j += EV_THREADS) po[j] = ps[j];
-    if (t == 0) p.counts[bh] = 0;
+  if (len <= p.budget) {                      // the whole cluster leaves
+    for (int j = c * EV_THREADS + t; j < len; j += nc * EV_THREADS) {
+      if (so != sc) so[j] = sc[j];
+      if (po != ps) po[j] = ps[j];
+    }
     return;
   }
-  __shared__ int hist[256];
-  __shared__ int2 warp_sums[EV_THREADS / 32];
-  __shared__ int s_always, s_digit, s_need;
-  const long long rf = (long long)p.next_pos[b] - p.n_recent;
-  const int recent_from = (int)max(-2147483648ll, rf);
-  if (t == 0) s_always = 0;
+  // this CTA's rows [j0, j0 + n), in words of 32
+  const int words_all = (len + 31) >> 5, wpc = (words_all + nc - 1) / nc;
+  const int j0 = min(c * wpc, words_all) * 32, n = min(len - j0, wpc * 32), nw = (n + 31) >> 5;
+  const int recent_from = (int)max(-2147483648ll, (long long)p.next_pos[b] - p.n_recent);
+  (&sh.hist[0][0])[t] = 0;                    // 2 x 256 bins, 512 threads
+  if (t == 0) sh.always = 0;
   __syncthreads();
-  int n = 0;
-  for (int j = t; j < len; j += EV_THREADS) n += ev_always(p, ps[j], recent_from);
-  atomicAdd(&s_always, n);
-  __syncthreads();
-  // the class the border lies in: the rows kept always when there are more of
-  // them than the budget, else the others
-  const bool among_always = s_always > p.budget;
-  int need = among_always ? p.budget : p.budget - s_always;
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    if (t < 256) hist[t] = 0;
-    __syncthreads();
-    for (int j = t; j < len; j += EV_THREADS) {
-      const uint32_t k = ev_key(sc[j]);
-      if (ev_always(p, ps[j], recent_from) == among_always && (shift == 24 || (k >> (shift + 8)) == prefix))
-        atomicAdd(&hist[(k >> shift) & 255], 1);
+  auto key_of = [&](int i) { return p.cached ? skey[i] : ev_key(sc[j0 + i]); };
+
+  // ---- read, and the first digit of the rows not kept always -------------------
+  int n_always = 0;
+  for (int w0 = warp; w0 < nw; w0 += 4 * EV_WARPS) {
+    float s[4];
+    int at[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = (w0 + u * EV_WARPS) * 32 + lane;
+      s[u] = i < n ? sc[j0 + i] : 0.f;
+      at[u] = i < n ? ps[j0 + i] : 0;
     }
-    __syncthreads();
-    if (t == 0) {      // the digit whose bin the need-th largest key falls into
-      int left = need, d = 255;
-      while (d > 0 && hist[d] < left) left -= hist[d--];
-      s_digit = d;
-      s_need = left;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int w = w0 + u * EV_WARPS, i = w * 32 + lane;
+      if (w >= nw) break;
+      const uint32_t k = ev_key(s[u]);
+      const bool in = i < n, al = in && (at[u] < p.n_sink || at[u] >= recent_from);
+      const uint32_t m = __ballot_sync(0xffffffffu, al);
+      if (lane == 0) always[w] = m;
+      n_always += __popc(m);
+      if (p.cached) skey[i] = k;
+      if (in && !al) atomicAdd(&sh.hist[0][k >> 24], 1);
     }
-    __syncthreads();
-    prefix = (prefix << 8) | s_digit;
-    need = s_need;
   }
-  // kept: class above the border, or key > prefix, or one of the first `need`
-  // rows with key == prefix
-  int* holes = p.lists + (long long)bh * 2 * p.max_moves;
-  int* from = holes + p.max_moves;
-  int ties = 0, nh = 0, nf = 0;
-  for (int j0 = 0; j0 < len; j0 += EV_THREADS) {
-    const int j = j0 + t;
-    bool keep = false, tie = false;
-    float s = 0.f;
-    int po_j = 0;
-    if (j < len) {
-      s = sc[j];
-      po_j = ps[j];
-      const uint32_t k = ev_key(s);
-      const bool al = ev_always(p, po_j, recent_from);
-      if (al != among_always) {
-        keep = al;
-      } else {
-        keep = k > prefix;
-        tie = k == prefix;
+  if (lane == 0 && n_always) atomicAdd(&sh.always, n_always);
+
+  // ---- radix select ---------------------------------------------------------------
+  // the class the border lies in: the others, or the rows kept always should they
+  // exceed the budget (the first digit is then counted again)
+  bool among_always = false, recount = false;
+  int need = 0, buf = 0;
+  uint32_t prefix = 0;
+  for (int shift = 24; shift >= 0;) {
+    if (shift < 24 || recount) {
+      for (int i = t; i < n; i += EV_THREADS) {
+        const uint32_t k = key_of(i);
+        if ((((always[i >> 5] >> (i & 31)) & 1) != 0) == among_always && (shift == 24 || (k >> (shift + 8)) == prefix))
+          atomicAdd(&sh.hist[buf][(k >> shift) & 255], 1);
       }
     }
-    int2 sum;
-    const int2 tr = ev_scan(make_int2(tie, 0), warp_sums, &sum);
-    if (tie) keep = ties + tr.x < need;
-    ties += sum.x;
-    const bool hole = j < p.budget && j < len && !keep, src = j >= p.budget && keep;
-    const int2 r = ev_scan(make_int2(hole, src), warp_sums, &sum);
-    if (hole) holes[nh + r.x] = j;
-    if (j < p.budget && keep) so[j] = s, po[j] = po_j;
-    nh += sum.x;
-    __syncthreads();                 // this chunk's holes are listed
-    if (src) {
-      const int to = holes[nf + r.y];
-      from[nf + r.y] = j;
-      so[to] = s;
-      po[to] = po_j;
+    cluster.sync();
+    if (shift == 24 && !recount) {
+      int al = lane < nc ? *cluster.map_shared_rank(&sh.always, lane) : 0;
+      al = __reduce_add_sync(0xffffffffu, al);
+      need = p.budget - al;
+      if (need < 0) {
+        need = p.budget;
+        among_always = recount = true;
+        buf = 1;
+        continue;
+      }
     }
-    nf += sum.y;
+    if (t < EV_BINS) {
+      int x = 0;
+#pragma unroll
+      for (int r = 0; r < EV_MAX_CLUSTER; ++r)
+        if (r < nc) x += cluster.map_shared_rank(&sh.hist[buf][0], r)[t];
+      sh.total[t] = x;
+      sh.hist[buf ^ 1][t] = 0;                // free: its readers passed the barrier above
+    }
+    __syncthreads();
+    // every warp: lane l has bins 8 l .. 8 l + 7; the digit's bin holds the need-th
+    // largest key (need 0: no row of this class, any digit does)
+    int cnt[8], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mine += cnt[i] = sh.total[8 * lane + i];
+    int above = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_down_sync(0xffffffffu, above, o);
+      if (lane + o < 32) above += u;
+    }
+    above -= mine;
+    int digit = -1, rest = 0;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+      if (above < need && above + cnt[i] >= need) digit = 8 * lane + i, rest = need - above;
+      above += cnt[i];
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, digit >= 0);
+    const int from = who ? __ffs(who) - 1 : 0;
+    digit = who ? __shfl_sync(0xffffffffu, digit, from) : 255;
+    need = who ? __shfl_sync(0xffffffffu, rest, from) : 0;
+    prefix = (prefix << 8) | (uint32_t)digit;
+    buf ^= 1;
+    shift -= 8;
   }
-  if (t == 0) p.counts[bh] = nf;
+
+  // ---- bitmaps: kept for certain, and ties at the border ------------------------------
+  for (int w = warp; w < nw; w += EV_WARPS) {
+    const int i = w * 32 + lane;
+    const uint32_t k = i < n ? key_of(i) : 0u;
+    const bool al = (always[w] >> lane) & 1, in_class = i < n && al == among_always;
+    const uint32_t m_tie = __ballot_sync(0xffffffffu, in_class && k == prefix);
+    const uint32_t m_keep = __ballot_sync(0xffffffffu, i < n && (in_class ? k > prefix : al));
+    if (lane == 0) tie[w] = m_tie, keep[w] = m_keep;
+  }
+  __syncthreads();
+  // thread t owns words [w_lo, w_hi); front(w): rows of word w before the budget
+  const int wpt = (nw + EV_THREADS - 1) / EV_THREADS, w_lo = min(nw, t * wpt), w_hi = min(nw, w_lo + wpt);
+  auto valid = [&](int w) { return n - w * 32 >= 32 ? 0xffffffffu : (1u << (n - w * 32)) - 1; };
+  auto front = [&](int w) {
+    const int m = p.budget - (j0 + w * 32);
+    return m >= 32 ? 0xffffffffu : m <= 0 ? 0u : (1u << m) - 1;
+  };
+  int ties = 0, ties_front = 0, sum, sum_front;
+  int leave = 0, stay = 0, sum_leave, sum_stay;
+  for (int w = w_lo; w < w_hi; ++w) {
+    const uint32_t f = front(w);
+    ties += __popc(tie[w]);
+    ties_front += __popc(tie[w] & f);
+    leave += __popc(~(keep[w] | tie[w]) & valid(w) & f);
+    stay += __popc(keep[w] & ~f);
+  }
+  ev_scan(sh, ties, ties_front, sum, sum_front);
+  ev_scan(sh, leave, stay, sum_leave, sum_stay);
+  if (t == 0) sh.border = make_int4(sum_front, sum - sum_front, sum_leave, sum_stay);
+  cluster.sync();
+  // lane r: CTA r's part.  Its ties are kept as far as `need` reaches after those
+  // of the CTAs before it, the ones before the budget first
+  int holes, srcs, moves;
+  {
+    const int4 x = lane < nc ? *cluster.map_shared_rank(&sh.border, lane) : make_int4(0, 0, 0, 0);
+    int before = x.x + x.y;
+#pragma unroll
+    for (int o = 1; o < EV_MAX_CLUSTER; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += u;
+    }
+    before -= x.x + x.y;
+    const int kept = max(0, min(need - before, x.x + x.y)), kept_front = min(kept, x.x);
+    int hr = x.z + x.x - kept_front, sr = x.w + kept - kept_front;      // holes and sources of CTA r
+    moves = __reduce_add_sync(0xffffffffu, sr);
+    holes = __reduce_add_sync(0xffffffffu, lane < c ? hr : 0);
+    srcs = __reduce_add_sync(0xffffffffu, lane < c ? sr : 0);
+    ties += __shfl_sync(0xffffffffu, before, c);                       // ties before this thread's words
+  }
+  int nh = 0, ns = 0;
+  for (int w = w_lo; w < w_hi; ++w) {
+    uint32_t m = tie[w], k = keep[w];
+    for (; m && ties < need; m &= m - 1, ++ties) k |= m & (0u - m);
+    ties += __popc(m);
+    keep[w] = k;
+    nh += base_h[w] = __popc(~k & valid(w) & front(w));
+    ns += base_s[w] = __popc(k & ~front(w));
+  }
+  ev_scan(sh, nh, ns, sum, sum_front);
+  holes += nh, srcs += ns;
+  for (int w = w_lo; w < w_hi; ++w) {
+    const int x = base_h[w], y = base_s[w];
+    base_h[w] = holes, base_s[w] = srcs;
+    holes += x, srcs += y;
+  }
+  __syncthreads();
+
+  // ---- the lists, and the rows that stay in place -----------------------------------
+  int* hole_list = p.lists + (long long)bh * 2 * p.max_moves;
+  int* src_list = hole_list + p.max_moves;
+  const uint32_t lt = (1u << lane) - 1;
+  for (int w = warp; w < nw; w += EV_WARPS) {
+    const int i = w * 32 + lane, j = j0 + i;
+    const uint32_t k = keep[w];
+    const bool kept = (k >> lane) & 1, front = j < p.budget;
+    const uint32_t m_h = __ballot_sync(0xffffffffu, i < n && front && !kept);
+    const uint32_t m_s = __ballot_sync(0xffffffffu, !front && kept);
+    if ((m_h >> lane) & 1) hole_list[base_h[w] + __popc(m_h & lt)] = j;
+    if ((m_s >> lane) & 1) src_list[base_s[w] + __popc(m_s & lt)] = j;
+    if (front && kept) {
+      if (so != sc) so[j] = sc[j];
+      if (po != ps) po[j] = ps[j];
+    }
+  }
+  cluster.sync();                             // lists complete; also the last read of a peer's shared memory
+
+  // ---- move ---------------------------------------------------------------------------
+  for (int i = c * EV_THREADS + t; i < moves; i += nc * EV_THREADS) {
+    const int from = src_list[i], to = hole_list[i];
+    so[to] = sc[from];
+    po[to] = ps[from];
+  }
+  const int vecs = p.head_bytes / 16;         // 16-byte pieces of a K row; as many of the V row
+  uint8_t* kb = p.kc + b * p.seq_bytes + (long long)h * p.head_bytes;
+  uint8_t* vb = p.vc + b * p.seq_bytes + (long long)h * p.head_bytes;
+  const int iters = (2 * vecs + 31) / 32, stride = nc * EV_WARPS;
+  const int mine = moves > c * EV_WARPS + warp ? (moves - (c * EV_WARPS + warp) + stride - 1) / stride : 0;
+  constexpr int U = 4;                        // pieces in flight per lane
+  for (int u0 = 0; u0 < mine * iters; u0 += U) {
+    uint4 x[U];
+    uint8_t* dst[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      dst[u] = nullptr;
+      const int unit = u0 + u, m = unit / iters, piece = (unit - m * iters) * 32 + lane;
+      if (m >= mine || piece >= 2 * vecs) continue;
+      const int at = c * EV_WARPS + warp + m * stride;
+      uint8_t* base = piece < vecs ? kb + piece * 16 : vb + (piece - vecs) * 16;
+      dst[u] = base + hole_list[at] * p.row_bytes;
+      x[u] = *(const uint4*)(base + src_list[at] * p.row_bytes);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (dst[u]) *(uint4*)dst[u] = x[u];
+  }
 }
 
-__global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(const EvictParams p, int rows_per_block) {
-  const int bh = blockIdx.y, b = bh / p.nkv, h = bh - b * p.nkv;
-  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0)
-    p.lens_out[b] = min(max(0, min(p.lens[b], p.max_len)), p.budget);
-  const int n = p.counts[bh];
-  const int r0 = blockIdx.x * rows_per_block, r1 = min(n, r0 + rows_per_block);
-  if (r0 >= r1) return;
-  const int* holes = p.lists + (long long)bh * 2 * p.max_moves;
-  const int* from = holes + p.max_moves;
-  const int vecs = p.head_bytes / 16;
-  uint8_t* base[2] = {p.kc + b * p.seq_bytes + (long long)h * p.head_bytes,
-                      p.vc + b * p.seq_bytes + (long long)h * p.head_bytes};
-  for (int i = threadIdx.x; i < (r1 - r0) * 2 * vecs; i += EV_MOVE_THREADS) {
-    const int row = i / (2 * vecs), c = i - row * 2 * vecs, kv = c >= vecs;
-    const long long off = (long long)(kv ? c - vecs : c) * 16;
-    const uint4 x = *(const uint4*)(base[kv] + from[r0 + row] * p.row_bytes + off);
-    *(uint4*)(base[kv] + holes[r0 + row] * p.row_bytes + off) = x;
-  }
+// lens_out in place: only once every cluster has read lens
+__global__ void evict_lens_kernel(int* lens, int batch, int max_len, int budget) {
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b < batch) lens[b] = min(max(0, min(lens[b], max_len)), budget);
 }
 
 namespace {
@@ -194,6 +349,8 @@ int evict_check(const InfernoEvict* e) {
   if ((long long)e->head_dim * es % 16 || e->head_dim > 8192)
     return set_error(INFERNO_EINVAL, "cache_evict: head_dim %d is not a multiple of 16 bytes or above 8192",
                      e->head_dim);
+  if (e->max_len > EV_MAX_LEN)
+    return set_error(INFERNO_EINVAL, "cache_evict: max_len %d is above %d", e->max_len, EV_MAX_LEN);
   if (e->budget < 1) return set_error(INFERNO_EINVAL, "cache_evict: budget %d", e->budget);
   if (e->n_sink < 0 || e->n_recent < 0 || (long long)e->n_sink + e->n_recent > e->budget)
     return set_error(INFERNO_EINVAL, "cache_evict: n_sink %d + n_recent %d exceed the budget %d", e->n_sink,
@@ -205,8 +362,7 @@ int evict_check(const InfernoEvict* e) {
 int evict_max_moves(const InfernoEvict* e) { return std::max(0, std::min(e->budget, e->max_len - e->budget)); }
 
 int64_t evict_workspace(const InfernoEvict* e) {
-  const int64_t n = (int64_t)e->batch * e->n_kv_heads;
-  return ((n * 4 + 255) / 256 + 1) * 256 + n * 2 * evict_max_moves(e) * 4;
+  return (int64_t)e->batch * e->n_kv_heads * 2 * evict_max_moves(e) * 4 + 256;
 }
 
 }  // namespace
@@ -257,23 +413,50 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.pos_out = e->slot_pos_out;
   p.lens_out = e->lens_out;
   p.stride = e->score_stride;
-  p.batch = e->batch;
   p.nkv = e->n_kv_heads;
   p.max_len = e->max_len;
   p.budget = e->budget;
   p.n_sink = e->n_sink;
   p.n_recent = e->n_recent;
   p.max_moves = evict_max_moves(e);
+  p.lists = (int*)workspace;
+  if (e->lens_out == e->lens) p.lens_out = nullptr;
+  // CTAs per (sequence, KV head): up to 8 while a CTA keeps 512 rows (fewer do not
+  // pay for the wider barriers) and all CTAs run at once, two per SM
   const int n = e->batch * e->n_kv_heads;
-  p.counts = (int*)workspace;
-  p.lists = (int*)((char*)workspace + ((size_t)n * 4 + 255) / 256 * 256);
+  int dev = 0;
+  INF_CUDA_TRY(cudaGetDevice(&dev));
+  int nc = 1;
+  while (nc < EV_MAX_CLUSTER && e->max_len >= nc * 2 * 512 && n * nc * 2 <= 2 * num_sms(dev)) nc *= 2;
+  auto smem_of = [&](int ctas, bool cached) {
+    const long long words = ((e->max_len + 31) / 32 + ctas - 1) / ctas;
+    return words * 4 * (5 + (cached ? 32 : 0));
+  };
+  while (nc < EV_MAX_CLUSTER && smem_of(nc, true) > EV_SMEM) nc *= 2;
+  p.cached = smem_of(nc, true) <= EV_SMEM;
+  p.words = ((e->max_len + 31) / 32 + nc - 1) / nc;
+  const size_t smem = smem_of(nc, p.cached);
   cudaStream_t st = (cudaStream_t)stream;
-  evict_select_kernel<<<n, EV_THREADS, 0, st>>>(p);
-  cudaError_t err = cudaGetLastError();
+  static DeviceOnce once;
+  cudaError_t err = once.run([] {
+    return cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
+  });
   if (err == cudaSuccess) {
-    const int rows = std::max(1, EV_MOVE_THREADS * 4 / (2 * p.head_bytes / 16));
-    const int bx = std::max(1, (p.max_moves + rows - 1) / rows);
-    evict_move_kernel<<<dim3(bx, n), EV_MOVE_THREADS, 0, st>>>(p, rows);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n * nc));
+    cfg.blockDim = dim3(EV_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = nc;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    err = cudaLaunchKernelEx(&cfg, evict_kernel, p);
+  }
+  if (err == cudaSuccess && !p.lens_out) {
+    evict_lens_kernel<<<(e->batch + 127) / 128, 128, 0, st>>>(e->lens_out, e->batch, e->max_len, e->budget);
     err = cudaGetLastError();
   }
   return err == cudaSuccess ? 0 : set_error(INFERNO_ECUDA, "cache_evict launch: %s", cudaGetErrorString(err));

@@ -2,10 +2,13 @@
 // (inferno_rope).
 //
 // A pair (a, b) of a head becomes (a cos - b sin, a sin + b cos) with the angle
-// positions[t] * f_i.  A block takes TB tokens (and a slice of their heads): its
-// threads first put cos and sin of the tokens' angles into shared memory, once
-// for all heads, then stream the heads through registers, one 16-byte vector
-// (two for the half layout, whose pairs lie rope_dim / 2 apart) per item.
+// positions[t] * f_i.  A block takes a few tokens: its threads first put cos and
+// sin of the tokens' angles into shared memory, once for all heads.  Then a team
+// of threads, one per 16-byte column of a head (a column of the half layout is two
+// vectors, rope_dim / 2 apart), takes four heads (or two) of a token at a time: cos and sin
+// of a column are read once for them, and the loads of all are in flight together.  (One vector per thread and index computation was bound by
+// instructions: 96 us for 16383 tokens x 40 heads of 128 bf16, and more items in
+// flight only made it slower.)
 //
 // Angles: f_i / (2 pi) is a double, so positions[t] * f_i / (2 pi) has the turn
 // exact to 2^-52 of itself; the whole turns are dropped in double and the rest,
@@ -45,42 +48,77 @@ struct RopeParams {
   long long qs, ks, vs, qos, kos, vos;   // elements between token rows
   const int *positions, *slots;
   const float* freq_factors;
-  int n_tokens, n_rows, head_dim, rope_dim;
+  int n_tokens, n_heads, n_kv, n_rows, head_dim, rope_dim;
   int tb;                                // tokens per block
-  uint32_t items;                        // items of one token (q, then k, then v)
-  uint32_t q_items, k_items;             // items of q alone, of q and k
-  uint32_t slice;                        // items of one block (over its tb tokens)
-  FastDiv by_items, by_head;             // items per token; items per head of q and k
-  uint32_t rot_items;                    // items of a head that are rotated
+  int cols, rot_cols;                    // columns of a head; those that are rotated
+  int teams;                             // teams of a block (cols threads each, at most a block)
+  uint32_t q_units, units;               // units (a few heads of one token): of q, of q and k
+  uint32_t slice;                        // units of one block (over its tb tokens)
+  uint32_t v_cols;                       // vectors of a v row (0: none)
+  uint32_t v_slice;                      // v vectors of one block (over its tb tokens)
+  FastDiv by_units, by_v;
   float gain, sign;                      // factor of cos and sin; -1: rotate back
   double turns[ROPE_MAX_PAIRS];          // f_i / (2 pi), without freq_factors
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f(T x) {
-  if constexpr (std::is_same_v<T, float>) return x;
-  else if constexpr (std::is_same_v<T, __half>) return __half2float(x);
-  else return __bfloat162float(x);
-}
-template <typename T>
-__device__ __forceinline__ T from_f(float x) {
-  if constexpr (std::is_same_v<T, float>) return x;
-  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(x);
-  else return __float2bfloat16_rn(x);
-}
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T x[V];
 };
 
-// V: elements of one access (the widest that sizes, strides and pointers
-// allow).  ILV: interleaved pairs; one item then holds whole pairs.
+// V elements <-> fp32, 16-bit types two at a time where there are two
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Vec<T, V>& v, float (&f)[V]) {
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = v.x[i];
+  } else if constexpr (V == 1) {
+    f[0] = (float)v.x[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      float2 y;
+      if constexpr (std::is_same_v<T, __half>) y = __half22float2(*(const __half2*)&v.x[i]);
+      else y = __bfloat1622float2(*(const __nv_bfloat162*)&v.x[i]);
+      f[i] = y.x, f[i + 1] = y.y;
+    }
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> pack(const float (&f)[V]) {
+  Vec<T, V> v;
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.x[i] = f[i];
+  } else if constexpr (V == 1) {
+    v.x[0] = (T)f[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      if constexpr (std::is_same_v<T, __half>) *(__half2*)&v.x[i] = __floats2half2_rn(f[i], f[i + 1]);
+      else *(__nv_bfloat162*)&v.x[i] = __floats2bfloat162_rn(f[i], f[i + 1]);
+    }
+  }
+  return v;
+}
+
+// Heads of a unit: four, but two where a column is two vectors of eight values,
+// whose 64 fp32 values of four heads leave too few registers for four blocks per
+// SM (16383 tokens x 40 heads of 128 bf16: 95 us with four, 74 us with two)
 template <typename T, int V, bool ILV>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constant__ RopeParams p) {
+__host__ __device__ constexpr int rope_heads() {
+  return V == 8 && !ILV ? 2 : 4;
+}
+
+// V: elements of one access (the widest that sizes, strides and pointers
+// allow).  ILV: interleaved pairs; a column then holds whole pairs.
+template <typename T, int V, bool ILV>
+__global__ void __launch_bounds__(ROPE_THREADS, 4) rope_kernel(const __grid_constant__ RopeParams p) {
   extern __shared__ float2 cs[];                     // [tb][rope_dim / 2] (cos, sin)
-  constexpr int RV = ILV && V < 2 ? 2 : V;           // values of one rotated vector
-  constexpr int NP = ILV ? RV / 2 : RV;              // pairs of one rotated item
   using Vt = Vec<T, V>;
+  constexpr bool TWO = !ILV || V == 1;               // a column is two vectors
+  constexpr int NP = ILV ? (V == 1 ? 1 : V / 2) : V; // pairs of one rotated column
+  constexpr int HB = rope_heads<T, V, ILV>();        // heads of a unit
   const int half = p.rope_dim >> 1;
   const int t0 = blockIdx.x * p.tb, nt = min(p.tb, p.n_tokens - t0);
   for (int i = threadIdx.x; i < nt * half; i += ROPE_THREADS) {
@@ -94,81 +132,94 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constan
     cs[i] = make_float2(cn * p.gain, sn * p.gain * p.sign);
   }
   __syncthreads();
-  const uint32_t end = min((blockIdx.y + 1) * p.slice, (uint32_t)nt * p.items);
-  constexpr int U = 2;                               // items in flight per thread
-  for (uint32_t e0 = blockIdx.y * p.slice + threadIdx.x; e0 < end; e0 += U * ROPE_THREADS) {
-    alignas(16) T a[U][RV];
-    alignas(16) T b[U][RV];
-    T* dst[U];
-    int pair[U];                                     // first pair, or -1: copied
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      dst[u] = nullptr;
-      const uint32_t e = e0 + u * ROPE_THREADS;
-      if (e >= end) continue;
-      const uint32_t tl = p.by_items.div(e);
-      uint32_t it = e - tl * p.items;
+
+  // ---- q and k ----
+  const int width = min(p.cols, ROPE_THREADS), team = threadIdx.x / width, col0 = threadIdx.x - team * width;
+  const uint32_t end = min((blockIdx.y + 1) * p.slice, (uint32_t)nt * p.units);
+  if (team < p.teams) {
+    for (uint32_t unit = blockIdx.y * p.slice + team; unit < end; unit += p.teams) {
+      const uint32_t tl = p.by_units.div(unit), u = unit - tl * p.units;
       const int t = t0 + (int)tl;
-      const T* src;
+      const bool isq = u < p.q_units;
+      const int h0 = (int)(isq ? u : u - p.q_units) * HB, nh = min(HB, (isq ? p.n_heads : p.n_kv) - h0);
       long long row = t;
-      if (it >= p.q_items && p.slots) {
+      if (!isq && p.slots) {
         row = __ldg(p.slots + t);
         if (row < 0 || row >= p.n_rows) continue;
       }
-      if (it >= p.k_items) {                         // v: copied whole
-        it -= p.k_items;
-        src = (const T*)p.v + (long long)t * p.vs + (long long)it * V;
-        dst[u] = (T*)p.vo + row * p.vos + (long long)it * V;
-        pair[u] = -1;
-      } else {
-        const bool isq = it < p.q_items;
-        if (!isq) it -= p.q_items;
-        const uint32_t h = p.by_head.div(it), j = it - h * p.by_head.d;
-        const bool rot = j < p.rot_items;
-        const long long off = (long long)h * p.head_dim +
-                              (rot ? (long long)j * RV : (long long)p.rope_dim + (long long)(j - p.rot_items) * V);
-        src = isq ? (const T*)p.q + (long long)t * p.qs + off : (const T*)p.k + (long long)t * p.ks + off;
-        dst[u] = isq ? (T*)p.qo + row * p.qos + off : (T*)p.ko + row * p.kos + off;
-        pair[u] = rot ? (int)(tl * half + j * NP) : -1;
-      }
-      if (pair[u] < 0) {
-        *(Vt*)a[u] = *(const Vt*)src;
-      } else {
+      const T* src0 = (isq ? (const T*)p.q + (long long)t * p.qs : (const T*)p.k + (long long)t * p.ks) + (long long)h0 * p.head_dim;
+      T* dst0 = (isq ? (T*)p.qo + row * p.qos : (T*)p.ko + row * p.kos) + (long long)h0 * p.head_dim;
+      for (int col = col0; col < p.cols; col += width) {
+        const bool rot = col < p.rot_cols;
+        const int off = !rot ? p.rope_dim + (col - p.rot_cols) * V : ILV ? 2 * NP * col : V * col;
+        const int second = ILV ? 1 : half;           // from a vector to its partner
+        const T* src = src0 + off;
+        T* dst = dst0 + off;
+        Vt a[HB], b[HB];
 #pragma unroll
-        for (int i = 0; i < RV; i += V) *(Vt*)(a[u] + i) = *(const Vt*)(src + i);
-        if constexpr (!ILV) *(Vt*)b[u] = *(const Vt*)(src + half);
+        for (int i = 0; i < HB; ++i)
+          if (i < nh) {
+            a[i] = *(const Vt*)(src + i * p.head_dim);
+            if (TWO && rot) b[i] = *(const Vt*)(src + i * p.head_dim + second);
+          }
+        if (!rot) {
+#pragma unroll
+          for (int i = 0; i < HB; ++i)
+            if (i < nh) *(Vt*)(dst + i * p.head_dim) = a[i];
+          continue;
+        }
+        float2 w[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) w[i] = cs[tl * half + col * NP + i];
+#pragma unroll
+        for (int i = 0; i < HB; ++i)
+          if (i < nh) {
+            float x[V], y[V];
+            unpack<T, V>(a[i], x);
+            if constexpr (TWO) {
+              unpack<T, V>(b[i], y);
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                const float xr = x[j] * w[j].x - y[j] * w[j].y;
+                y[j] = x[j] * w[j].y + y[j] * w[j].x;
+                x[j] = xr;
+              }
+              *(Vt*)(dst + i * p.head_dim + second) = pack<T, V>(y);
+            } else {
+#pragma unroll
+              for (int j = 0; j < NP; ++j) {
+                const float xr = x[2 * j] * w[j].x - x[2 * j + 1] * w[j].y;
+                x[2 * j + 1] = x[2 * j] * w[j].y + x[2 * j + 1] * w[j].x;
+                x[2 * j] = xr;
+              }
+            }
+            *(Vt*)(dst + i * p.head_dim) = pack<T, V>(x);
+          }
       }
     }
+  }
+
+  // ---- v: copied ----
+  if (!p.v_cols) return;
+  const uint32_t v_end = min((blockIdx.y + 1) * p.v_slice, (uint32_t)nt * p.v_cols);
+  for (uint32_t e0 = blockIdx.y * p.v_slice + threadIdx.x; e0 < v_end; e0 += HB * ROPE_THREADS) {
+    Vt x[HB];
+    T* dst[HB];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!dst[u]) continue;
-      if (pair[u] < 0) {
-        *(Vt*)dst[u] = *(const Vt*)a[u];
-        continue;
-      }
-      const float2* w = cs + pair[u];
-      if constexpr (ILV) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const float2 c = w[i];
-          const float x = to_f(a[u][2 * i]), y = to_f(a[u][2 * i + 1]);
-          a[u][2 * i] = from_f<T>(x * c.x - y * c.y);
-          a[u][2 * i + 1] = from_f<T>(x * c.y + y * c.x);
-        }
-#pragma unroll
-        for (int i = 0; i < RV; i += V) *(Vt*)(dst[u] + i) = *(const Vt*)(a[u] + i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const float2 c = w[i];
-          const float x = to_f(a[u][i]), y = to_f(b[u][i]);
-          a[u][i] = from_f<T>(x * c.x - y * c.y);
-          b[u][i] = from_f<T>(x * c.y + y * c.x);
-        }
-        *(Vt*)dst[u] = *(const Vt*)a[u];
-        *(Vt*)(dst[u] + half) = *(const Vt*)b[u];
-      }
+    for (int i = 0; i < HB; ++i) {
+      dst[i] = nullptr;
+      const uint32_t e = e0 + i * ROPE_THREADS;
+      if (e >= v_end) continue;
+      const uint32_t tl = p.by_v.div(e), c = e - tl * p.v_cols;
+      const int t = t0 + (int)tl;
+      const long long row = __ldg(p.slots + t);
+      if (row < 0 || row >= p.n_rows) continue;
+      dst[i] = (T*)p.vo + row * p.vos + (long long)c * V;
+      x[i] = *(const Vt*)((const T*)p.v + (long long)t * p.vs + (long long)c * V);
     }
+#pragma unroll
+    for (int i = 0; i < HB; ++i)
+      if (dst[i]) *(Vt*)dst[i] = x[i];
   }
 }
 
@@ -301,18 +352,21 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
   p.slots = r->slots;
   p.freq_factors = r->freq_factors;
   p.n_tokens = r->n_tokens;
+  p.n_heads = has_q ? r->n_heads : 0;
+  p.n_kv = has_k ? r->n_kv_heads : 0;
   p.n_rows = r->n_rows;
   p.head_dim = r->head_dim;
   p.rope_dim = r->rope_dim;
   const int half = r->rope_dim / 2;
-  const int rv = ilv && vec < 2 ? 2 : vec;
-  p.rot_items = (ilv ? r->rope_dim : half) / rv;
-  const uint32_t per_head = p.rot_items + (r->head_dim - r->rope_dim) / vec;
-  p.q_items = has_q ? r->n_heads * per_head : 0;
-  p.k_items = p.q_items + (has_k ? r->n_kv_heads * per_head : 0);
-  p.items = p.k_items + (has_v ? (uint32_t)(kw / vec) : 0);
-  p.by_head = FastDiv(per_head);
-  p.by_items = FastDiv(p.items);
+  p.rot_cols = ilv ? r->rope_dim / std::max(vec, 2) : half / vec;
+  p.cols = p.rot_cols + (r->head_dim - r->rope_dim) / vec;
+  p.teams = std::max(1, ROPE_THREADS / p.cols);
+  const int hb = vec == 8 && !ilv ? rope_heads<__half, 8, false>() : rope_heads<float, 4, false>();
+  p.q_units = (p.n_heads + hb - 1) / hb;
+  p.units = p.q_units + (p.n_kv + hb - 1) / hb;
+  p.v_cols = has_v ? (uint32_t)(kw / vec) : 0;
+  p.by_units = FastDiv(std::max(1u, p.units));
+  p.by_v = FastDiv(std::max(1u, p.v_cols));
   p.sign = r->inverse ? -1.0f : 1.0f;
   p.gain = r->mscale != 0.0f ? r->mscale
            : r->scaling == INFERNO_ROPE_SCALE_PARTS && r->factor > 1.0f ? (float)(0.1 * std::log((double)r->factor) + 1.0)
@@ -339,22 +393,23 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
     p.turns[i] = g;
   }
 
-  // tokens per block: enough that every thread has an angle to compute, fewer
-  // when there are too few tokens to fill the SMs; then slices of about eight
-  // items per thread, down to one per thread when there are few
+  // tokens per block: about four units for every team, fewer when there are too
+  // few tokens to give every SM two blocks; then the units of a block are cut into
+  // slices (which compute the angles again) until there are
   int dev = 0;
   INF_CUDA_TRY(cudaGetDevice(&dev));
   const long long sms = num_sms(dev);
-  long long tb = std::max(1, ROPE_THREADS / half);
-  tb = std::max(1ll, std::min(tb, r->n_tokens / (2 * sms)));
-  while (tb > 1 && tb * p.items > (1ll << 30)) tb /= 2;
+  const long long work = std::max<long long>(p.units, (p.v_cols + (long long)hb * p.cols - 1) / ((long long)hb * p.cols));
+  long long tb = 1;
+  while (tb < 16 && tb * work < 4ll * p.teams && tb * 2 * half <= 1024) tb *= 2;
+  while (tb > 1 && (r->n_tokens + tb - 1) / tb < 2 * sms) tb /= 2;
   p.tb = (int)tb;
   const long long blocks = (r->n_tokens + tb - 1) / tb;
-  const long long per_block = tb * p.items;
-  long long per_thread = std::min(8ll, std::max(1ll, blocks * per_block / (2 * sms * ROPE_THREADS)));
-  long long slices = (per_block + per_thread * ROPE_THREADS - 1) / (per_thread * ROPE_THREADS);
+  long long slices = std::max(1ll, std::min((2 * sms + blocks - 1) / blocks, (tb * work + p.teams - 1) / p.teams));
+  slices = std::max(slices, (tb * work + 64ll * p.teams - 1) / (64ll * p.teams));
   slices = std::min(slices, 65535ll);
-  p.slice = (uint32_t)((per_block + slices - 1) / slices);
+  p.slice = (uint32_t)((tb * p.units + slices - 1) / slices);
+  p.v_slice = (uint32_t)((tb * p.v_cols + slices - 1) / slices);
   const dim3 grid((unsigned)blocks, (unsigned)slices);
   const size_t smem = (size_t)tb * half * sizeof(float2);
   cudaStream_t st = (cudaStream_t)stream;

@@ -42,14 +42,19 @@ class _Sized(C.Structure):
     """A parameter struct whose struct_size is filled in."""
 
     def __init__(self, **kw):
-        super().__init__(**kw)
-        self.struct_size = C.sizeof(self)
+        C.Structure.__init__(self, self._size, **kw)      # struct_size is the first field
+
+
+def _sized(cls):
+    cls._size = C.sizeof(cls)
+    return cls
 
 
 def _fields(kind, names):
     return [(n, kind) for n in names.split()]
 
 
+@_sized
 class InfernoRope(_Sized):
     """include/inferno_b200.h InfernoRope (rotary positions with cache append)."""
     _fields_ = (_fields(C.c_int32, "struct_size type n_tokens n_heads n_kv_heads head_dim rope_dim layout scaling "
@@ -59,6 +64,7 @@ class InfernoRope(_Sized):
                 + _fields(C.c_int64, "q_stride k_stride v_stride q_out_stride k_out_stride v_out_stride"))
 
 
+@_sized
 class InfernoAttention(_Sized):
     """include/inferno_b200.h InfernoAttention (shared prefix + per-sequence caches)."""
     _fields_ = (_fields(C.c_int32, "struct_size type batch n_tokens n_heads n_kv_heads head_dim prefix_len max_len")
@@ -66,6 +72,7 @@ class InfernoAttention(_Sized):
                 + _fields(C.c_void_p, "q prefix_k prefix_v k_cache v_cache lens scores out"))
 
 
+@_sized
 class InfernoEvict(_Sized):
     """include/inferno_b200.h InfernoEvict (cache eviction by gathered weight)."""
     _fields_ = (_fields(C.c_int32, "struct_size type batch n_kv_heads head_dim max_len budget n_sink n_recent reserved")

@@ -413,6 +413,13 @@ def test_evict_more_kept_always_than_budget():
     _check_evict(tid, k, v, scores, pos, [1200], [1200], budget=300, n_sink=1, n_recent=0)
 
 
+@pytest.mark.parametrize("rows,budget", [(40000, 9000), (400000, 100000)])
+def test_evict_long(rows, budget):
+    """Parts of a cluster that hold their keys in shared memory, and ones too long for it."""
+    tid, k, v, scores, pos = _evict_case("bf16", 1, 1, 8, rows, seed=7)
+    _check_evict(tid, k, v, scores, pos, [rows - 3], [rows], budget=budget, n_sink=4, n_recent=budget // 3)
+
+
 def test_evict_strides_and_max_len():
     tid, dt = R.TYPES["f16"]
     g = _gen(2)
