@@ -31,9 +31,10 @@ namespace inf {
 namespace {
 
 constexpr int AC_KT = 16;                       // keys per tile
-constexpr int AC_SMEM = 227 * 1024;
+constexpr int AC_SMEM = 227 * 1024, AC_SMEM_HALF = 113 * 1024;
 constexpr int AC_FIN_THREADS = 256;
-constexpr int AC_FIN_SLOTS = AC_FIN_THREADS;    // own rows per finishing CTA
+constexpr int AC_FIN_PER = 4;                   // own rows per thread of a finishing CTA
+constexpr int AC_FIN_SLOTS = AC_FIN_THREADS * AC_FIN_PER;
 
 template <typename T>
 struct AcType;
@@ -50,10 +51,15 @@ struct AcGeo {
   static constexpr int ROW = HD * (int)sizeof(T);              // bytes of a K / V row of one head
   static constexpr int ITEM = AC_KT * ROW;                     // bytes of a ring slot
   static constexpr int QBYTES = AcType<T>::F32 ? 16 * R * ROW : 0;
-  // eight warps (512 threads could not hold the accumulators of head_dim 256);
-  // fewer groups where three slots each would not fit
-  static constexpr int NG0 = 8 / R;
-  static constexpr int ROOM = AC_SMEM - 1024 - QBYTES;
+  // two CTAs of four warps per SM, so that one streams while the other starts or
+  // merges; one CTA of up to eight warps where the half SM does not hold three
+  // slots per group (fp32 at head_dim 256)
+  static constexpr int ML = 8 * 16 * 8;
+  static constexpr bool TWO = (4 / R) * 3 * ITEM + QBYTES + ML <= AC_SMEM_HALF &&
+                              4 * 16 * HD * 4 + QBYTES + ML <= AC_SMEM_HALF;   // ring and merge buffer share their space
+  static constexpr int CTAS = TWO ? 2 : 1;
+  static constexpr int ROOM = (TWO ? AC_SMEM_HALF : AC_SMEM) - ML - QBYTES;
+  static constexpr int NG0 = (TWO ? 4 : 8) / R;
   static constexpr int NG = NG0 * 3 * ITEM <= ROOM ? NG0 : NG0 / 2;
   static constexpr int NW = NG * R;
   static constexpr int THREADS = NW * 32;
@@ -62,7 +68,7 @@ struct AcGeo {
   static constexpr int RING = NG * SLOTS * ITEM;
   static constexpr int MERGE = NW * 16 * HD * 4;
   static constexpr int SMEM = QBYTES + (RING > MERGE ? RING : MERGE) + NW * 16 * 8;
-  static_assert(SLOTS >= 3 && SMEM <= AC_SMEM, "shared memory");
+  static_assert(SLOTS >= 3 && SMEM <= (TWO ? AC_SMEM_HALF : AC_SMEM), "shared memory");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -157,7 +163,7 @@ __device__ __forceinline__ float ac_weight(float2 ml, float M) {
 }
 
 template <typename T, int HD, int R>
-__global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(const __grid_constant__ AcParams p, int prefix_part, int row_tiles) {
+__global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTAS) ac_part_kernel(const __grid_constant__ AcParams p, int prefix_part, int row_tiles) {
   using G = AcGeo<T, HD, R>;
   constexpr bool F32 = AcType<T>::F32;
   constexpr int ROW = G::ROW, ITEM = G::ITEM, SLOTS = G::SLOTS, GT = R * 32;
@@ -166,6 +172,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(co
   const int grp = warp / R, rt = warp - grp * R;       // key group, row tile of the warp
   const int gtid = tid - grp * GT;                     // thread within the group
 
+  pdl_trigger();
   AcWork w;
   {
     int x = blockIdx.x;
@@ -198,7 +205,10 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(co
     w.k += (long long)w.kvh * ROW;
     w.v += (long long)w.kvh * ROW;
   }
-  if (w.j0 >= w.j1) return;          // nothing of this sequence in this split
+  if (w.j0 >= w.j1) {                // nothing of this sequence in this split
+    pdl_wait();
+    return;
+  }
   const long long key_stride = (long long)p.nkv * ROW;
 
   const uint32_t s_q = smem_u32(smem);                            // fp32 only: [16 R][HD]
@@ -315,11 +325,17 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(co
 #pragma unroll
       for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] = c[0][a >> 2][a & 3] + c[1][a >> 2][a & 3];
     } else {
-      float c[2][3][4];              // per n tile: hi hi, hi lo, lo hi
+      // The tensor core truncates when it adds to its accumulator, so a long chain
+      // drifts by half a step of the sum per product.  Chains are kept to four
+      // products and added up in fp32 (rounded): 1.6e-6 -> 5e-7 of the result.
+      float lo[2][4];                // hi lo and lo hi: small, one chain
 #pragma unroll
-      for (int a = 0; a < 24; ++a) c[a / 12][(a / 4) % 3][a & 3] = 0.f;
+      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] = lo[a >> 2][a & 3] = 0.f;
 #pragma unroll
-      for (int cg = 0; cg < HD / 32; ++cg)
+      for (int cg = 0; cg < HD / 32; ++cg) {
+        float c[2][4];
+#pragma unroll
+        for (int a = 0; a < 8; ++a) c[a >> 2][a & 3] = 0.f;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           // four consecutive dims per thread, used as the k indices t4 and t4 + 4
@@ -341,14 +357,17 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(co
               uint32_t h0, h1, l0, l1;
               split_tf32(kv[st][n][0], h0, l0);
               split_tf32(kv[st][n][1], h1, l1);
-              mma_tf32(c[n][0], ah, h0, h1);
-              mma_tf32(c[n][1], ah, l0, l1);
-              mma_tf32(c[n][2], al, h0, h1);
+              mma_tf32(c[n], ah, h0, h1);
+              mma_tf32(lo[n], ah, l0, l1);
+              mma_tf32(lo[n], al, h0, h1);
             }
           }
         }
 #pragma unroll
-      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] = c[a >> 2][0][a & 3] + (c[a >> 2][1][a & 3] + c[a >> 2][2][a & 3]);
+        for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] += c[a >> 2][a & 3];
+      }
+#pragma unroll
+      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] += lo[a >> 2][a & 3];
     }
     // ---- running softmax ----
     float mx_lo = -INFINITY, mx_hi = -INFINITY;
@@ -422,7 +441,10 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(co
         split_tf32(s[n][3], ph[n][3], pl[n][3]);
       }
 #pragma unroll
-      for (int cg = 0; cg < HD / 32; ++cg)
+      for (int cg = 0; cg < HD / 32; ++cg) {
+        float c[4][4];               // this tile's share, added to O in fp32 (see S)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) c[x >> 2][x & 3] = 0.f;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           // dims 32 cg + 4 g + x are column g of n tile 4 cg + x
@@ -434,11 +456,14 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(co
             uint32_t h0, h1, l0, l1;
             split_tf32(a[x], h0, l0);
             split_tf32(b[x], h1, l1);
-            mma_tf32(o[4 * cg + x], ph[n], h0, h1);
-            mma_tf32(o[4 * cg + x], ph[n], l0, l1);
-            mma_tf32(o[4 * cg + x], pl[n], h0, h1);
+            mma_tf32(c[x], ph[n], l0, l1);
+            mma_tf32(c[x], pl[n], h0, h1);
+            mma_tf32(c[x], ph[n], h0, h1);
           }
         }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[4 * cg + (x >> 2)][x & 3] += c[x >> 2][x & 3];
+      }
     }
   }
 
@@ -504,6 +529,9 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, 1) ac_part_kernel(co
       p.part_ml[at] = make_float2(M, L);
     }
   }
+  // launched beside the prefix part: not complete before it, so that the
+  // finishing kernel, which waits for this one, finds both
+  pdl_wait();
 }
 
 // splits of a row that hold something: all of the prefix, own ones up to lens
@@ -535,6 +563,7 @@ __device__ __forceinline__ float2 ac_row_stats(const AcParams& p, long long row,
 template <typename T, int HD>
 __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_constant__ AcParams p, int row_blocks, int slot_blocks) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
   if (blockIdx.x < row_blocks) {
     const long long row = (long long)blockIdx.x * (AC_FIN_THREADS / 32) + warp;
     const long long tok = row / p.nh;
@@ -546,6 +575,7 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
     float a[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) a[i] = 0.f;
+#pragma unroll 4
     for (int s = 0; s < n; ++s) {
       const float f = ac_weight(p.part_ml[row * p.n_splits + s], st.x);
       const float* o = p.part_o + (row * p.n_splits + s) * HD + lane * PER;
@@ -566,30 +596,48 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
     return;
   }
   constexpr int CHUNK = 64;                          // rows whose statistics are held at once
+  constexpr int U = 4;                               // rows whose logits are in flight
   __shared__ float2 st[CHUNK];
+  __shared__ long long at[CHUNK];                    // the rows' logits
   const int x = blockIdx.x - row_blocks, bh = x / slot_blocks, b = bh / p.nkv, kvh = bh - b * p.nkv;
-  const int j = (x - bh * slot_blocks) * AC_FIN_SLOTS + threadIdx.x;
+  const int j0 = (x - bh * slot_blocks) * AC_FIN_SLOTS + threadIdx.x;
   const int len = max(0, min(p.lens[b], p.max_len));
-  if (j - (int)threadIdx.x >= len) return;
+  if (j0 - (int)threadIdx.x >= len) return;
   const int n = ac_live_splits(p, b), rows = p.n_tok * p.group;
-  float sum = 0.f;
+  float sum[AC_FIN_PER];
+#pragma unroll
+  for (int i = 0; i < AC_FIN_PER; ++i) sum[i] = 0.f;
   for (int r0 = 0; r0 < rows; r0 += CHUNK) {
     const int nr = min(CHUNK, rows - r0);
     __syncthreads();
     for (int r = warp; r < nr; r += AC_FIN_THREADS / 32) {
       const int t = (r0 + r) / p.group, h = kvh * p.group + (r0 + r) - t * p.group;
-      const float2 s = ac_row_stats(p, (long long)(b * p.n_tok + t) * p.nh + h, n);
-      if (lane == 0) st[r] = s;
+      const long long row = (long long)(b * p.n_tok + t) * p.nh + h;
+      const float2 s = ac_row_stats(p, row, n);
+      if (lane == 0) st[r] = s, at[r] = row * p.logit_stride;
     }
     __syncthreads();
-    if (j < len)
-      for (int r = 0; r < nr; ++r) {
-        const int t = (r0 + r) / p.group, h = kvh * p.group + (r0 + r) - t * p.group;
-        const float lg = p.logits[((long long)(b * p.n_tok + t) * p.nh + h) * p.logit_stride + j];
-        if (lg != -INFINITY) sum += exp2f(lg - st[r].x) * st[r].y;
-      }
+    for (int r = 0; r < nr; r += U) {
+      float lg[U][AC_FIN_PER];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < AC_FIN_PER; ++i) {
+          const int j = j0 + i * AC_FIN_THREADS;
+          lg[u][i] = r + u < nr && j < len ? p.logits[at[r + u] + j] : -INFINITY;
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < AC_FIN_PER; ++i)
+          if (lg[u][i] != -INFINITY) sum[i] += exp2f(lg[u][i] - st[r + u].x) * st[r + u].y;
+    }
   }
-  if (j < len) p.scores[(long long)bh * p.score_stride + j] += sum;
+#pragma unroll
+  for (int i = 0; i < AC_FIN_PER; ++i) {
+    const int j = j0 + i * AC_FIN_THREADS;
+    if (j < len) p.scores[(long long)bh * p.score_stride + j] += sum[i];
+  }
 }
 
 // ---- host ---------------------------------------------------------------------
@@ -602,20 +650,24 @@ struct AcPlan {
 
 int ac_row_class(long long rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
-// Splits of `len` keys for `units` CTAs' worth of other work: enough CTAs for
-// `waves` per SM, but at least 128 keys (eight tiles of 16) each, and at most 256
-void ac_split(long long units, int len, int waves, int* splits, int* split_len) {
+// Splits of `len` keys when `units` (KV heads x row tiles x sequences) share the
+// GPU: about four rounds of two CTAs per SM, which evens out ragged lengths, as
+// long as a split keeps 256 keys (below that starting and merging a CTA costs more
+// than it streams); with fewer keys, one round, down to 64 keys, one tile of 16
+// for each of the four key groups.
+void ac_split(long long units, long long len, int* splits, int* split_len) {
   if (len <= 0) {
     *splits = 0;
-    *split_len = 16;
+    *split_len = 64;
     return;
   }
-  long long want = std::max(1ll, (148ll * waves + units - 1) / units);
-  want = std::min(want, 256ll);
-  int sl = (int)((len + want - 1) / want);
-  sl = std::max(128, (sl + 127) / 128 * 128);
-  *split_len = sl;
-  *splits = (len + sl - 1) / sl;
+  auto keys = [&](long long ctas) {
+    const long long want = std::max(1ll, std::min(256ll, ctas / units));
+    return ((len + want - 1) / want + 63) / 64 * 64;
+  };
+  const long long sl = std::max(keys(4 * 296), std::min(256ll, keys(296)));
+  *split_len = (int)sl;
+  *splits = (int)((len + sl - 1) / sl);
 }
 
 int ac_check(const InfernoAttention* a) {
@@ -654,8 +706,8 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   pl.p_r = ac_row_class(pre);
   pl.o_tiles = (int)((own + 16 * pl.o_r - 1) / (16 * pl.o_r));
   pl.p_tiles = (int)((pre + 16 * pl.p_r - 1) / (16 * pl.p_r));
-  ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, 1, &p->p_splits, &p->p_split_len);
-  ac_split((long long)pl.o_tiles * a->n_kv_heads * a->batch, a->max_len, 2, &p->o_splits, &p->o_split_len);
+  ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, &p->p_splits, &p->p_split_len);
+  ac_split((long long)pl.o_tiles * a->n_kv_heads * a->batch, a->max_len, &p->o_splits, &p->o_split_len);
   p->n_splits = p->p_splits + p->o_splits;
   p->logit_stride = a->scores ? ((long long)a->max_len + 15) / 16 * 16 : 0;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
@@ -665,37 +717,60 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   return pl;
 }
 
+// beside: may start while the kernel before it in the call still runs (it waits
+// for that one itself)
+template <typename... Args, typename... Given>
+cudaError_t ac_launch(void (*kernel)(Args...), long long blocks, int threads, size_t smem, cudaStream_t st, bool beside,
+                      Given... args) {
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <typename T, int HD, int R>
-cudaError_t ac_launch_part(const AcParams& p, int prefix_part, int tiles, long long blocks, cudaStream_t st) {
+cudaError_t ac_launch_part(const AcParams& p, int prefix_part, int tiles, long long blocks, bool beside, cudaStream_t st) {
   using G = AcGeo<T, HD, R>;
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(ac_part_kernel<T, HD, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
   });
   if (e != cudaSuccess) return e;
-  ac_part_kernel<T, HD, R><<<(unsigned)blocks, G::THREADS, G::SMEM, st>>>(p, prefix_part, tiles);
-  return cudaGetLastError();
+  return ac_launch(ac_part_kernel<T, HD, R>, blocks, G::THREADS, G::SMEM, st, beside, p, prefix_part, tiles);
 }
 template <typename T, int HD>
-cudaError_t ac_part(const AcParams& p, int r, int prefix_part, int tiles, cudaStream_t st) {
+cudaError_t ac_part(const AcParams& p, int r, int prefix_part, int tiles, bool beside, cudaStream_t st) {
   const long long blocks = (long long)tiles * p.nkv * (prefix_part ? p.p_splits : (long long)p.o_splits * p.batch);
-  if (blocks <= 0) return cudaSuccess;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  return r == 1   ? ac_launch_part<T, HD, 1>(p, prefix_part, tiles, blocks, st)
-         : r == 2 ? ac_launch_part<T, HD, 2>(p, prefix_part, tiles, blocks, st)
-                  : ac_launch_part<T, HD, 4>(p, prefix_part, tiles, blocks, st);
+  return r == 1   ? ac_launch_part<T, HD, 1>(p, prefix_part, tiles, blocks, beside, st)
+         : r == 2 ? ac_launch_part<T, HD, 2>(p, prefix_part, tiles, blocks, beside, st)
+                  : ac_launch_part<T, HD, 4>(p, prefix_part, tiles, blocks, beside, st);
 }
 template <typename T, int HD>
 cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
-  cudaError_t e = ac_part<T, HD>(p, pl.p_r, 1, pl.p_tiles, st);
-  if (e == cudaSuccess) e = ac_part<T, HD>(p, pl.o_r, 0, pl.o_tiles, st);
+  cudaError_t e = cudaSuccess;
+  bool any = false;                    // a kernel of this call is in flight
+  if (p.p_splits) {
+    e = ac_part<T, HD>(p, pl.p_r, 1, pl.p_tiles, false, st);
+    any = true;
+  }
+  if (e == cudaSuccess && p.o_splits) {
+    e = ac_part<T, HD>(p, pl.o_r, 0, pl.o_tiles, any, st);
+    any = true;
+  }
   if (e != cudaSuccess) return e;
   const long long row_blocks = (pl.rows + AC_FIN_THREADS / 32 - 1) / (AC_FIN_THREADS / 32);
   const long long slot_blocks = p.scores ? (p.max_len + AC_FIN_SLOTS - 1) / AC_FIN_SLOTS : 0;
   const long long blocks = row_blocks + slot_blocks * p.batch * p.nkv;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  ac_finish_kernel<T, HD><<<(unsigned)blocks, AC_FIN_THREADS, 0, st>>>(p, (int)row_blocks, (int)std::max(1ll, slot_blocks));
-  return cudaGetLastError();
+  return ac_launch(ac_finish_kernel<T, HD>, blocks, AC_FIN_THREADS, 0, st, any, p, (int)row_blocks,
+                   (int)std::max(1ll, slot_blocks));
 }
 template <typename T>
 cudaError_t ac_run_hd(int hd, const AcParams& p, const AcPlan& pl, cudaStream_t st) {
