@@ -235,7 +235,8 @@ int inferno_device_error(int device, int clear) {
   if (cudaMemcpy(&v, w, sizeof v, cudaMemcpyDeviceToHost) != cudaSuccess)
     return set_error(INFERNO_ECUDA, "reading device error word failed");
   if (clear) cudaMemset(w, 0, sizeof(int));
-  return v;
+  const int a = attn_prefix_device_error(device, clear);
+  return v ? v : a;
 }
 
 int inferno_dequantize(int ggml_type, const void* src, int64_t n, float* dst, void* stream) {

@@ -642,6 +642,7 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
 
 // ---- host ---------------------------------------------------------------------
 struct AcPlan {
+  bool p_tc;                      // prefix part on tcgen05
   int p_r, o_r;                   // 16-row tiles per CTA of the two parts
   int p_tiles, o_tiles;           // row tiles
   long long rows;                 // query rows over all heads
@@ -669,6 +670,9 @@ void ac_split(long long units, long long len, int* splits, int* split_len) {
   *split_len = (int)sl;
   *splits = (int)((len + sl - 1) / sl);
 }
+
+// The prefix part on tcgen05: 16-bit types with more rows than two tiles of 16
+bool ac_prefix_tc(int type, long long rows) { return type != INFERNO_F32 && rows > 32; }
 
 int ac_check(const InfernoAttention* a) {
   if (!a) return set_error(INFERNO_EINVAL, "attention_cached: null parameters");
@@ -706,7 +710,18 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   pl.p_r = ac_row_class(pre);
   pl.o_tiles = (int)((own + 16 * pl.o_r - 1) / (16 * pl.o_r));
   pl.p_tiles = (int)((pre + 16 * pl.p_r - 1) / (16 * pl.p_r));
-  ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, &p->p_splits, &p->p_split_len);
+  pl.p_tc = ac_prefix_tc(a->type, pre);
+  if (pl.p_tc) {
+    // one round of CTAs: splits of at least two tiles
+    pl.p_tiles = (int)((pre + ap_rows() - 1) / ap_rows());
+    const long long units = (long long)pl.p_tiles * a->n_kv_heads;
+    const long long want = std::max(1ll, std::min(256ll, 148ll * ap_ctas_per_sm(a->head_dim) / units));
+    const long long sl = ((a->prefix_len + want - 1) / want + 63) / 64 * 64;
+    p->p_split_len = (int)std::max(128ll, sl);
+    p->p_splits = (a->prefix_len + p->p_split_len - 1) / p->p_split_len;
+  } else {
+    ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, &p->p_splits, &p->p_split_len);
+  }
   ac_split((long long)pl.o_tiles * a->n_kv_heads * a->batch, a->max_len, &p->o_splits, &p->o_split_len);
   p->n_splits = p->p_splits + p->o_splits;
   p->logit_stride = a->scores ? ((long long)a->max_len + 15) / 16 * 16 : 0;
@@ -756,8 +771,8 @@ cudaError_t ac_part(const AcParams& p, int r, int prefix_part, int tiles, bool b
 template <typename T, int HD>
 cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
-  bool any = false;                    // a kernel of this call is in flight
-  if (p.p_splits) {
+  bool any = pl.p_tc && p.p_splits;    // a kernel of this call is in flight
+  if (p.p_splits && !pl.p_tc) {
     e = ac_part<T, HD>(p, pl.p_r, 1, pl.p_tiles, false, st);
     any = true;
   }
@@ -839,6 +854,7 @@ extern "C" int inferno_attention_cached(const InfernoAttention* a, void* workspa
   p.part_ml = (float2*)((char*)workspace + pl.off_ml);
   p.logits = (float*)((char*)workspace + pl.off_logits);
   cudaStream_t st = (cudaStream_t)stream;
+  if (pl.p_tc && p.p_splits && (rc = launch_attn_prefix_tc(a->type, a->head_dim, p, pl.p_tiles, st))) return rc;
   const cudaError_t e = a->type == INFERNO_F32   ? ac_run_hd<float>(a->head_dim, p, pl, st)
                         : a->type == INFERNO_F16 ? ac_run_hd<__half>(a->head_dim, p, pl, st)
                                                  : ac_run_hd<__nv_bfloat16>(a->head_dim, p, pl, st);

@@ -30,4 +30,9 @@ struct AcParams {
 
 constexpr float AC_LOG2E = 1.4426950408889634f;
 
+// the prefix part on tcgen05 (attn_prefix_tc.cu): query rows per CTA, CTAs per SM
+int ap_rows();
+int ap_ctas_per_sm(int hd);
+int launch_attn_prefix_tc(int type, int hd, const AcParams& p, int row_tiles, cudaStream_t st);
+
 }  // namespace inf

@@ -203,5 +203,7 @@ int launch_embed_row(int type, const void* W, long long row_bytes, int inner, co
 
 // device error word of the library (per device)
 int* device_error_word(int device);
+// the same of the tcgen05 prefix attention, which needs none allocated
+int attn_prefix_device_error(int device, int clear);
 
 }  // namespace inf
