@@ -30,6 +30,15 @@ struct AcParams {
 
 constexpr float AC_LOG2E = 1.4426950408889634f;
 
+// 16 bytes to shared memory, zeros where not valid (src is then not read)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // the prefix part on tcgen05 (attn_prefix_tc.cu): query rows per CTA, CTAs per SM
 int ap_rows();
 int ap_ctas_per_sm(int hd);

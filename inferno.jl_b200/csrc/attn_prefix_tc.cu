@@ -47,8 +47,9 @@ struct ApGeo {
   static constexpr int CTAS = HD == 256 ? 1 : 2;
 };
 
+// A poll sleeps for up to about 4 us, so this gives up after about two seconds.
 __device__ __forceinline__ bool ap_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 22); ++i)
+  for (uint32_t i = 0; i < (1u << 19); ++i)
     if (mbar_try_wait(bar, parity)) return true;
   atomicExch(&ap_error, DERR_MBAR_TIMEOUT);
   return false;
@@ -128,8 +129,9 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
   uint64_t* v_empty = v_full + ST;
   uint64_t* s_full = v_empty + ST;        // 2
   uint64_t* p_full = s_full + 2;          // 2
-  uint64_t* pv_done = p_full + 2;         // 1
-  uint64_t* q_full = pv_done + 1;         // 1
+  uint64_t* pv_done = p_full + 2;         // 1: phase j is P V of tile j
+  uint64_t* o_done = pv_done + 1;         // 1: all of them
+  uint64_t* q_full = o_done + 1;          // 1
   uint32_t* s_tmem = (uint32_t*)(q_full + 1);
 
   int x = blockIdx.x;
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       mbar_init(&p_full[i], AP_M);
     }
     mbar_init(pv_done, 1);
+    mbar_init(o_done, 1);
     mbar_init(q_full, AP_M);
     fence_mbar_init();
   }
@@ -233,22 +236,24 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         umma_commit(pv_done);
         umma_commit(&v_empty[j % ST]);
       }
-      // no MMA in flight when TMEM is freed
-      if (!ok) ap_wait(pv_done, (tiles - 1) & 1);
+      umma_commit(o_done);
+      if (!ok) ap_wait(o_done, 0);          // no MMA in flight when TMEM is freed
     }
     __syncwarp();
   } else {
     // ================= softmax: one row per thread =================
-    for (int id = tid; id < AP_M * HD / 8; id += AP_M) {
-      const int r = id / (HD / 8), c = id % (HD / 8);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row0 + r < nrows) {
-        const int per_b = p.n_tok * p.group, rr = row0 + r, b = rr / per_b, tg = rr - b * per_b, t = tg / p.group;
-        v = *(const uint4*)((const T*)p.q + (long long)(b * p.n_tok + t) * p.q_stride +
-                            (long long)(kvh * p.group + tg - t * p.group) * HD + c * 8);
-      }
-      *(uint4*)(s_q + (c >> 3) * AP_M * 128 + sw128_off(r, c & 7)) = v;
+    // a thread's 16-byte column is the same in all its rows; all copies in flight
+    constexpr int CH = HD / 8, STEP = AP_M / CH;
+    const int c = tid % CH, per_b = p.n_tok * p.group;
+#pragma unroll 8
+    for (int r = tid / CH; r < AP_M; r += STEP) {
+      const int rr = min(row0 + r, nrows - 1), b = rr / per_b, tg = rr - b * per_b, t = tg / p.group;
+      const T* src = (const T*)p.q + (long long)(b * p.n_tok + t) * p.q_stride +
+                     (long long)(kvh * p.group + tg - t * p.group) * HD + c * 8;
+      cp_async16(smem_u32(s_q) + (c >> 3) * AP_M * 128 + sw128_off(r, c & 7), src, row0 + r < nrows);
     }
+    cp_commit();
+    cp_wait<0>();
     fence_proxy_async_smem();
     mbar_arrive(q_full);
 
@@ -341,28 +346,42 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       mbar_arrive(&p_full[j & 1]);
     }
     // ---- partial result ----
-    // P V of the last two tiles may be in flight, and a parity names a phase only
-    // once the one before it is over
-    ok = ok && (tiles == 1 || ap_wait(pv_done, (tiles - 2) & 1)) && ap_wait(pv_done, (tiles - 1) & 1);
+    // its own barrier: pv_done may be one or two phases on by now, and a parity
+    // tells a phase only from its neighbours
+    ok = ok && ap_wait(o_done, 0);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
-      const int r = row0 + tid;
-      const bool in = r < nrows;
-      const int per_b = p.n_tok * p.group, b = r / per_b, tg = r - b * per_b, t = tg / p.group;
-      const long long row = (long long)(b * p.n_tok + t) * p.nh + kvh * p.group + (tg - t * p.group);
-      const long long at = row * p.n_splits + split;
+      // O leaves by whole 128-byte lines: 32 columns of a warp's 32 rows turn through
+      // shared memory (the K ring, idle now; 36 floats apart, so that neither side
+      // of the turn has two lanes of a phase on one bank), eight lanes per row
+      float* turn = (float*)s_k + warp * 32 * 36;
+      const int per_b = p.n_tok * p.group;
+      long long at[8];                                  // this lane's rows lane / 8 + 4 i
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = row0 + warp * 32 + i * 4 + (lane >> 3);
+        const int b = r / per_b, tg = r - b * per_b, t = tg / p.group;
+        at[i] = r < nrows ? ((long long)(b * p.n_tok + t) * p.nh + kvh * p.group + (tg - t * p.group)) * p.n_splits + split : -1;
+      }
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
+        __syncwarp();
         tmem_ld_x32(t_o + lane_base + c, o);
         tmem_wait_ld();
-        if (in) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *(uint4*)(p.part_o + at * HD + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
+        for (int i = 0; i < 32; i += 4) *(uint4*)(turn + lane * 36 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (at[i] >= 0)
+            *(uint4*)(p.part_o + at[i] * HD + c + (lane & 7) * 4) = *(const uint4*)(turn + (i * 4 + (lane >> 3)) * 36 + (lane & 7) * 4);
       }
-      if (in) p.part_ml[at] = make_float2(m, l);
+      const int r = row0 + tid;
+      if (r < nrows) {
+        const int b = r / per_b, tg = r - b * per_b, t = tg / p.group;
+        p.part_ml[((long long)(b * p.n_tok + t) * p.nh + kvh * p.group + (tg - t * p.group)) * p.n_splits + split] = make_float2(m, l);
+      }
     }
   }
   tc_fence_before();

@@ -274,6 +274,17 @@ def test_attention_extremes(dtype):
     _check_attn(tid, c, L)
 
 
+@pytest.mark.parametrize("dtype,kv,d,scale", [("bf16", 1, 128, 0.0), ("f16", 2, 64, -0.4), ("bf16", 1, 256, 0.1)])
+def test_attention_prefix_maximum_rises(dtype, kv, d, scale):
+    """Many query rows on a prefix whose logits grow along it, so that the running
+    maximum rises by far more than the slack again and again, in some rows only."""
+    tid, c, L = _attn_case(dtype, 24, 2, 4 * kv, kv, d, 3000, 40, [40 - b for b in range(24)])
+    c["pk"] *= torch.linspace(0.05, 6, 3000, device="cuda")[:, None, None].to(c["pk"].dtype)
+    c["q"][::3] *= 0.01
+    _check_attn(tid, c, L, scale)
+    assert lib().inferno_device_error(0, 0) == 0
+
+
 def test_attention_nan_rows_stay_apart():
     """A NaN in one sequence's rows makes that sequence's heads NaN, no others."""
     tid, c, L = _attn_case("bf16", 3, 1, 4, 2, 64, 100, 60, [60, 60, 60])
@@ -295,6 +306,7 @@ def test_attention_repeats_bit_for_bit():
         for _ in range(3):
             R.attention(a, ws)
             assert torch.equal(c["out"], first)
+        assert lib().inferno_device_error(0, 0) == 0
 
 
 def test_attention_captured_reads_lengths_on_the_device():
