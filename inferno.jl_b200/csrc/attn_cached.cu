@@ -550,38 +550,71 @@ __device__ __forceinline__ float2 ac_row_stats(const AcParams& p, long long row,
   return make_float2(M, L > 0.f ? 1.f / L : (L == L ? 0.f : L));
 }
 
-// blocks [0, row_blocks): one warp per row joins its splits; blocks behind:
-// `scores` of one (sequence, KV head), AC_FIN_SLOTS own rows each
-template <typename T, int HD>
+// blocks [0, row_blocks): W warps per row join its splits (every W-th one each,
+// then one another's sums in warp order), all loads of a warp in flight; blocks
+// behind: `scores` of one (sequence, KV head), AC_FIN_SLOTS own rows each
+template <typename T, int HD, int W>
 __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_constant__ AcParams p, int row_blocks, int slot_blocks) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int WARPS = AC_FIN_THREADS / 32;
   pdl_wait();
   if (blockIdx.x < row_blocks) {
-    const long long row = (long long)blockIdx.x * (AC_FIN_THREADS / 32) + warp;
-    const long long tok = row / p.nh;
-    const int h = (int)(row - tok * p.nh);
-    if (tok >= (long long)p.batch * p.n_tok) return;
-    const int n = ac_live_splits(p, (int)(tok / p.n_tok));
-    const float2 st = ac_row_stats(p, row, n);
     constexpr int PER = HD / 32;                     // dims of a lane
+    constexpr int U = 16 / PER < 4 ? 4 : 16 / PER;   // splits in flight
+    __shared__ float part[W > 1 ? WARPS : 1][HD];
+    const long long row = (long long)blockIdx.x * (WARPS / W) + warp / W;
+    const long long tok = row / p.nh;
+    const int h = (int)(row - tok * p.nh), sub = warp % W;
+    const bool live = tok < (long long)p.batch * p.n_tok;
+    if (W == 1 && !live) return;
     float a[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) a[i] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float f = ac_weight(p.part_ml[row * p.n_splits + s], st.x);
-      const float* o = p.part_o + (row * p.n_splits + s) * HD + lane * PER;
+    float inv = 0.f;
+    if (live) {
+      const int n = ac_live_splits(p, (int)(tok / p.n_tok));
+      const float2 st = ac_row_stats(p, row, n);
+      inv = st.y;
+      const float2* ml = p.part_ml + row * p.n_splits;
+      const float* o = p.part_o + row * p.n_splits * HD + lane * PER;
+      for (int s0 = sub; s0 < n; s0 += U * W) {
+        float f[U], x[U][PER];
 #pragma unroll
-      for (int i = 0; i < PER; i += 2) {
-        const float2 x = *(const float2*)(o + i);
-        a[i] = fmaf(f, x.x, a[i]);
-        a[i + 1] = fmaf(f, x.y, a[i + 1]);
+        for (int u = 0; u < U; ++u) {
+          const int s = s0 + u * W;
+          f[u] = 0.f;
+          if (s < n) {
+            f[u] = ac_weight(ml[s], st.x);
+#pragma unroll
+            for (int i = 0; i < PER; i += 2) {
+              const float2 y = *(const float2*)(o + (long long)s * HD + i);
+              x[u][i] = y.x, x[u][i + 1] = y.y;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) x[u][i] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < PER; ++i) a[i] = fmaf(f[u], x[u][i], a[i]);
       }
+    }
+    if constexpr (W > 1) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) part[warp][lane * PER + i] = a[i];
+      __syncthreads();
+      if (sub || !live) return;
+#pragma unroll
+      for (int w = 1; w < W; ++w)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) a[i] += part[warp + w][lane * PER + i];
     }
     T* out = (T*)p.out + tok * p.out_stride + (long long)h * HD + lane * PER;
 #pragma unroll
     for (int i = 0; i < PER; i += 2) {
-      const float x = a[i] * st.y, y = a[i + 1] * st.y;
+      const float x = a[i] * inv, y = a[i + 1] * inv;
       if constexpr (AcType<T>::F32) *(float2*)(out + i) = make_float2(x, y);
       else *(uint32_t*)(out + i) = pack2<T>(x, y);
     }
@@ -773,11 +806,14 @@ cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
     any = true;
   }
   if (e != cudaSuccess) return e;
-  const long long row_blocks = (pl.rows + AC_FIN_THREADS / 32 - 1) / (AC_FIN_THREADS / 32);
+  // four warps per row when it has more splits than one warp has in flight
+  const bool wide = p.n_splits > 8;
+  const int per_block = AC_FIN_THREADS / 32 / (wide ? 4 : 1);
+  const long long row_blocks = (pl.rows + per_block - 1) / per_block;
   const long long slot_blocks = p.scores ? (p.max_len + AC_FIN_SLOTS - 1) / AC_FIN_SLOTS : 0;
   const long long blocks = row_blocks + slot_blocks * p.batch * p.nkv;
-  return ac_launch(ac_finish_kernel<T, HD>, blocks, AC_FIN_THREADS, 0, st, any, p, (int)row_blocks,
-                   (int)std::max(1ll, slot_blocks));
+  return ac_launch(wide ? ac_finish_kernel<T, HD, 4> : ac_finish_kernel<T, HD, 1>, blocks, AC_FIN_THREADS, 0, st, any, p,
+                   (int)row_blocks, (int)std::max(1ll, slot_blocks));
 }
 template <typename T>
 cudaError_t ac_run_hd(int hd, const AcParams& p, const AcPlan& pl, cudaStream_t st) {
