@@ -15,6 +15,8 @@
 // 16 rows cannot fill the 128-row tcgen05 instruction and the kernel is bound by
 // bytes; fp32 operands are carried as tf32 pairs (hi, lo) in three products,
 // about 21 significant bits.  The groups merge in shared memory.
+// ac_vec_kernel: the same for fp32 and few query rows, on the CUDA cores, a lane
+// holding some dims of the rows and of the keys (see there).
 // ac_finish_kernel: joins the splits of a row, and adds the weights of the own
 // rows to `scores` from the logits that the first kernel left.
 #include <algorithm>
@@ -154,6 +156,43 @@ __device__ __forceinline__ float ac_weight(float2 ml, float M) {
   return ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - M);
 }
 
+// the work of this CTA: rows_per_cta rows of a KV head against one split
+template <typename T, int HD>
+__device__ __forceinline__ AcWork ac_work(const AcParams& p, int prefix_part, int row_tiles, int rows_per_cta) {
+  AcWork w;
+  constexpr int ROW = HD * (int)sizeof(T);
+  int x = blockIdx.x;
+  const int splits = prefix_part ? p.p_splits : p.o_splits;
+  w.split = x % splits;
+  x /= splits;
+  w.row0 = (x % row_tiles) * rows_per_cta;
+  x /= row_tiles;
+  w.kvh = x % p.nkv;
+  x /= p.nkv;
+  const int rows = p.n_tok * p.group;
+  if (prefix_part) {
+    w.b = -1;
+    w.nrows = p.batch * rows;
+    w.len = p.prefix_len;
+    w.j0 = w.split * p.p_split_len;
+    w.j1 = min(w.len, w.j0 + p.p_split_len);
+    w.k = (const uint8_t*)p.pk;
+    w.v = (const uint8_t*)p.pv;
+  } else {
+    w.b = x;
+    w.nrows = rows;
+    w.len = max(0, min(p.lens[x], p.max_len));
+    w.j0 = w.split * p.o_split_len;
+    w.j1 = min(w.len, w.j0 + p.o_split_len);
+    w.k = (const uint8_t*)p.kc + (long long)x * p.seq_stride * (int)sizeof(T);
+    w.v = (const uint8_t*)p.vc + (long long)x * p.seq_stride * (int)sizeof(T);
+    w.split += p.p_splits;
+  }
+  w.k += (long long)w.kvh * ROW;
+  w.v += (long long)w.kvh * ROW;
+  return w;
+}
+
 template <typename T, int HD, int R>
 __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTAS) ac_part_kernel(const __grid_constant__ AcParams p, int prefix_part, int row_tiles) {
   using G = AcGeo<T, HD, R>;
@@ -165,38 +204,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
   const int gtid = tid - grp * GT;                     // thread within the group
 
   pdl_trigger();
-  AcWork w;
-  {
-    int x = blockIdx.x;
-    const int splits = prefix_part ? p.p_splits : p.o_splits;
-    w.split = x % splits;
-    x /= splits;
-    w.row0 = (x % row_tiles) * 16 * R;
-    x /= row_tiles;
-    w.kvh = x % p.nkv;
-    x /= p.nkv;
-    const int rows = p.n_tok * p.group;
-    if (prefix_part) {
-      w.b = -1;
-      w.nrows = p.batch * rows;
-      w.len = p.prefix_len;
-      w.j0 = w.split * p.p_split_len;
-      w.j1 = min(w.len, w.j0 + p.p_split_len);
-      w.k = (const uint8_t*)p.pk;
-      w.v = (const uint8_t*)p.pv;
-    } else {
-      w.b = x;
-      w.nrows = rows;
-      w.len = max(0, min(p.lens[x], p.max_len));
-      w.j0 = w.split * p.o_split_len;
-      w.j1 = min(w.len, w.j0 + p.o_split_len);
-      w.k = (const uint8_t*)p.kc + (long long)x * p.seq_stride * (int)sizeof(T);
-      w.v = (const uint8_t*)p.vc + (long long)x * p.seq_stride * (int)sizeof(T);
-      w.split += p.p_splits;
-    }
-    w.k += (long long)w.kvh * ROW;
-    w.v += (long long)w.kvh * ROW;
-  }
+  const AcWork w = ac_work<T, HD>(p, prefix_part, row_tiles, 16 * R);
   if (w.j0 >= w.j1) {                // nothing of this sequence in this split
     pdl_wait();
     return;
@@ -526,6 +534,181 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
   pdl_wait();
 }
 
+// ---- fp32, few rows -------------------------------------------------------------
+// A warp takes RN query rows and tiles of 32 / RN keys.  Lane l holds the dims
+// 4 l .. 4 l + 3 (and 128 + those; 2 l, 2 l + 1 at head_dim 64) of the rows, and
+// loads those of each key straight into registers: whole rows, coalesced, with no
+// shared memory between.  The 32 partial products of a tile (keys x rows) are
+// summed over the lanes by halving: at each of five steps a lane passes on half of
+// its values and keeps the other half, so 31 exchanges leave lane l with the logit
+// of key l / RN and row l % RN.  V's loads are in flight during S, the next K's
+// during P V.  At four rows a tile of head_dim 256 takes about 400 instructions for
+// 16 KB, a seventh of an SM's issue slots at the memory's rate; the tensor cores
+// would spend three tf32 products of 16 rows each on it (fp32, two sequences of
+// 65536 rows, four query rows: 253 us there).
+constexpr int AV_WARPS = 4;
+constexpr int AV_MAX_ROWS = 16;
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*(unsigned long long*)&a), "l"(*(unsigned long long*)&b), "l"(*(unsigned long long*)&c));
+  return *(float2*)&d;
+}
+
+template <int HD, int RN>
+__global__ void __launch_bounds__(AV_WARPS * 32, 2) ac_vec_kernel(const __grid_constant__ AcParams p, int prefix_part, int row_tiles) {
+  constexpr int KT = 32 / RN;                      // keys of a tile
+  constexpr int D2 = HD / 64;                      // float2 of a lane
+  __shared__ float merge[AV_WARPS][RN][HD];
+  __shared__ float2 s_ml[AV_WARPS][RN];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_trigger();
+  const AcWork w = ac_work<float, HD>(p, prefix_part, row_tiles, RN);
+  if (w.j0 >= w.j1) {
+    pdl_wait();
+    return;
+  }
+  const long long key_stride = (long long)p.nkv * HD;
+  // dims of float2 i of this lane: pairs (0, 1) and (2, 3) are one 16-byte access
+  auto dim = [&](int i) { return HD == 64 ? 2 * lane : 128 * (i >> 1) + 4 * lane + 2 * (i & 1); };
+  auto load = [&](const float* src, bool ok, float2 (&x)[D2]) {
+    if constexpr (HD == 64) {
+      x[0] = ok ? *(const float2*)(src + 2 * lane) : make_float2(0.f, 0.f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < D2; i += 2) {
+        const float4 y = ok ? *(const float4*)(src + dim(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[i] = make_float2(y.x, y.y);
+        x[i + 1] = make_float2(y.z, y.w);
+      }
+    }
+  };
+  auto load_tile = [&](const uint8_t* base, int key0, float2 (&x)[KT][D2]) {
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+      load((const float*)base + (long long)(key0 + k < w.j1 ? key0 + k : w.j0) * key_stride, key0 + k < w.j1, x[k]);
+  };
+  float2 kx[KT][D2], vx[KT][D2];
+  int key0 = w.j0 + warp * KT;
+  load_tile(w.k, key0, kx);
+  load_tile(w.v, key0, vx);
+
+  float2 q[RN][D2], o[RN][D2];
+#pragma unroll
+  for (int r = 0; r < RN; ++r) {
+    int b, t, h;
+    ac_row(p, w, min(w.row0 + r, w.nrows - 1), b, t, h);
+    load((const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD, w.row0 + r < w.nrows, q[r]);
+#pragma unroll
+    for (int i = 0; i < D2; ++i) o[r][i] = make_float2(0.f, 0.f);
+  }
+  // this lane's key and row of a tile
+  const int my_key = lane / RN, my_row = lane % RN;
+  int lim = 0;
+  float* lg = nullptr;
+  if (w.row0 + my_row < w.nrows) {
+    int b, t, h;
+    ac_row(p, w, w.row0 + my_row, b, t, h);
+    lim = w.b < 0 ? w.len : w.len - p.n_tok + 1 + t;
+    if (p.scores && w.b >= 0) lg = p.logits + ((long long)(b * p.n_tok + t) * p.nh + h) * p.logit_stride;
+  }
+  float m = -INFINITY, l = 0.f;
+
+  for (; key0 < w.j1; key0 += AV_WARPS * KT) {
+    // ---- S = Q K^T ----
+    float s[32];
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int r = 0; r < RN; ++r) {
+        float2 a = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < D2; ++i) a = fma2(kx[k][i], q[r][i], a);
+        s[k * RN + r] = a.x + a.y;
+      }
+    load_tile(w.k, key0 + AV_WARPS * KT, kx);
+#pragma unroll
+    for (int st = 16; st >= 1; st >>= 1) {
+      const bool up = lane & st;
+#pragma unroll
+      for (int i = 0; i < st; ++i) {
+        const float give = up ? s[i] : s[i + st], keep = up ? s[i + st] : s[i];
+        s[i] = keep + __shfl_xor_sync(0xffffffffu, give, st);
+      }
+    }
+    // ---- running softmax of row my_row ----
+    const int key = key0 + my_key;
+    const float x = key < w.j1 && key < lim ? s[0] * p.scale_log2 : -INFINITY;
+    if (lg && key < w.j1) lg[key] = x;
+    float mx = x;
+#pragma unroll
+    for (int of = RN; of < 32; of <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, of));
+    if (__any_sync(0xffffffffu, mx > m)) {
+      const float n = fmaxf(m, mx), f = n == -INFINITY ? 1.f : exp2f(m - n);
+      m = n;
+      l *= f;
+#pragma unroll
+      for (int r = 0; r < RN; ++r) {
+        const float g = __shfl_sync(0xffffffffu, f, r);
+#pragma unroll
+        for (int i = 0; i < D2; ++i) o[r][i].x *= g, o[r][i].y *= g;
+      }
+    }
+    const float pr = exp2f(x - (m == -INFINITY ? 0.f : m));
+    l += pr;
+    // ---- O += P V ----
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int r = 0; r < RN; ++r) {
+        const float g = __shfl_sync(0xffffffffu, pr, k * RN + r);
+#pragma unroll
+        for (int i = 0; i < D2; ++i) o[r][i] = fma2(make_float2(g, g), vx[k][i], o[r][i]);
+      }
+    load_tile(w.v, key0 + AV_WARPS * KT, vx);
+  }
+  // ---- merge the warps ----
+#pragma unroll
+  for (int of = RN; of < 32; of <<= 1) l += __shfl_xor_sync(0xffffffffu, l, of);
+  if (lane < RN) s_ml[warp][lane] = make_float2(m, l);
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < RN; ++r) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < AV_WARPS; ++x) M = fmaxf(M, s_ml[x][r].x);
+    const float f = ac_weight(s_ml[warp][r], M);
+#pragma unroll
+    for (int i = 0; i < D2; ++i) *(float2*)&merge[warp][r][dim(i)] = make_float2(o[r][i].x * f, o[r][i].y * f);
+  }
+  __syncthreads();
+  const int live = min(RN, w.nrows - w.row0);
+  for (int id = tid; id < live * (HD / 4); id += AV_WARPS * 32) {
+    const int r = id / (HD / 4), c = id % (HD / 4);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < AV_WARPS; ++x) {
+      const float4 y = *(const float4*)&merge[x][r][4 * c];
+      a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
+    }
+    int b, t, h;
+    ac_row(p, w, w.row0 + r, b, t, h);
+    const long long at = ((long long)(b * p.n_tok + t) * p.nh + h) * p.n_splits + w.split;
+    *(float4*)(p.part_o + at * HD + 4 * c) = a;
+    if (c == 0) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int x = 0; x < AV_WARPS; ++x) M = fmaxf(M, s_ml[x][r].x);
+#pragma unroll
+      for (int x = 0; x < AV_WARPS; ++x) L += s_ml[x][r].y * ac_weight(s_ml[x][r], M);
+      p.part_ml[at] = make_float2(M, L);
+    }
+  }
+  pdl_wait();                          // see ac_part_kernel
+}
+
 // splits of a row that hold something: all of the prefix, own ones up to lens
 __device__ __forceinline__ int ac_live_splits(const AcParams& p, int b) {
   int n = p.p_splits;
@@ -668,13 +851,18 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
 // ---- host ---------------------------------------------------------------------
 struct AcPlan {
   bool p_tc;                      // prefix part on tcgen05
-  int p_r, o_r;                   // 16-row tiles per CTA of the two parts
+  int p_r, o_r;                   // rows per CTA of the two parts: 16, 32, 64 (ac_part_kernel), 4, 8 (ac_vec_kernel)
   int p_tiles, o_tiles;           // row tiles
   long long rows;                 // query rows over all heads
   size_t off_ml, off_logits, bytes;
 };
 
-int ac_row_class(long long rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// Rows per CTA for a part with `rows` query rows per KV head: fp32 with few rows
+// goes to ac_vec_kernel in tiles of 4 or 8
+int ac_row_class(int type, long long rows) {
+  if (type == INFERNO_F32 && rows <= AV_MAX_ROWS) return rows <= 4 ? 4 : 8;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
 
 // Splits of `len` keys when `units` (KV heads x row tiles x sequences) share the
 // GPU: about four rounds of two CTAs per SM, which evens out ragged lengths, as
@@ -731,10 +919,10 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   p->max_len = a->max_len;
   const long long own = (long long)a->n_tokens * p->group, pre = own * a->batch;
   pl.rows = pre * a->n_kv_heads;
-  pl.o_r = ac_row_class(own);
-  pl.p_r = ac_row_class(pre);
-  pl.o_tiles = (int)((own + 16 * pl.o_r - 1) / (16 * pl.o_r));
-  pl.p_tiles = (int)((pre + 16 * pl.p_r - 1) / (16 * pl.p_r));
+  pl.o_r = ac_row_class(a->type, own);
+  pl.p_r = ac_row_class(a->type, pre);
+  pl.o_tiles = (int)((own + pl.o_r - 1) / pl.o_r);
+  pl.p_tiles = (int)((pre + pl.p_r - 1) / pl.p_r);
   pl.p_tc = ac_prefix_tc(a->type, pre);
   if (pl.p_tc) {
     // one round of CTAs: splits of at least two tiles
@@ -789,9 +977,13 @@ cudaError_t ac_launch_part(const AcParams& p, int prefix_part, int tiles, long l
 template <typename T, int HD>
 cudaError_t ac_part(const AcParams& p, int r, int prefix_part, int tiles, bool beside, cudaStream_t st) {
   const long long blocks = (long long)tiles * p.nkv * (prefix_part ? p.p_splits : (long long)p.o_splits * p.batch);
-  return r == 1   ? ac_launch_part<T, HD, 1>(p, prefix_part, tiles, blocks, beside, st)
-         : r == 2 ? ac_launch_part<T, HD, 2>(p, prefix_part, tiles, blocks, beside, st)
-                  : ac_launch_part<T, HD, 4>(p, prefix_part, tiles, blocks, beside, st);
+  if constexpr (AcType<T>::F32) {
+    if (r == 4) return ac_launch(ac_vec_kernel<HD, 4>, blocks, AV_WARPS * 32, 0, st, beside, p, prefix_part, tiles);
+    if (r == 8) return ac_launch(ac_vec_kernel<HD, 8>, blocks, AV_WARPS * 32, 0, st, beside, p, prefix_part, tiles);
+  }
+  return r == 16   ? ac_launch_part<T, HD, 1>(p, prefix_part, tiles, blocks, beside, st)
+         : r == 32 ? ac_launch_part<T, HD, 2>(p, prefix_part, tiles, blocks, beside, st)
+                   : ac_launch_part<T, HD, 4>(p, prefix_part, tiles, blocks, beside, st);
 }
 template <typename T, int HD>
 cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
