@@ -90,16 +90,16 @@ __device__ __forceinline__ float4 lds_f4(uint32_t a) {
 template <typename T>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<T, __half>)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -139,13 +139,12 @@ struct AcWork {
 
 // row `r` of a part (prefix: over all sequences) -> (b, t, h)
 __device__ __forceinline__ void ac_row(const AcParams& p, const AcWork& w, int r, int& b, int& t, int& h) {
-  const int per_b = p.n_tok * p.group;
   b = w.b;
   if (b < 0) {
-    b = r / per_b;
-    r -= b * per_b;
+    b = (int)p.by_seq.div(r);
+    r -= b * (int)p.by_seq.d;
   }
-  t = r / p.group;
+  t = (int)p.by_group.div(r);
   h = w.kvh * p.group + (r - t * p.group);
 }
 
@@ -156,12 +155,19 @@ __device__ __forceinline__ float ac_weight(float2 ml, float M) {
   return ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - M);
 }
 
+// blocks of a launch: the prefix part's, then the own part's; row tiles of each
+struct AcGrid {
+  int p_blocks, p_tiles, o_tiles;
+};
+
 // the work of this CTA: rows_per_cta rows of a KV head against one split
 template <typename T, int HD>
-__device__ __forceinline__ AcWork ac_work(const AcParams& p, int prefix_part, int row_tiles, int rows_per_cta) {
+__device__ __forceinline__ AcWork ac_work(const AcParams& p, AcGrid gr, int rows_per_cta) {
   AcWork w;
   constexpr int ROW = HD * (int)sizeof(T);
-  int x = blockIdx.x;
+  const bool prefix_part = (int)blockIdx.x < gr.p_blocks;
+  int x = prefix_part ? blockIdx.x : blockIdx.x - gr.p_blocks;
+  const int row_tiles = prefix_part ? gr.p_tiles : gr.o_tiles;
   const int splits = prefix_part ? p.p_splits : p.o_splits;
   w.split = x % splits;
   x /= splits;
@@ -194,7 +200,7 @@ __device__ __forceinline__ AcWork ac_work(const AcParams& p, int prefix_part, in
 }
 
 template <typename T, int HD, int R>
-__global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTAS) ac_part_kernel(const __grid_constant__ AcParams p, int prefix_part, int row_tiles) {
+__global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTAS) ac_part_kernel(const __grid_constant__ AcParams p, AcGrid gr) {
   using G = AcGeo<T, HD, R>;
   constexpr bool F32 = AcType<T>::F32;
   constexpr int ROW = G::ROW, ITEM = G::ITEM, SLOTS = G::SLOTS, GT = R * 32;
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
   const int gtid = tid - grp * GT;                     // thread within the group
 
   pdl_trigger();
-  const AcWork w = ac_work<T, HD>(p, prefix_part, row_tiles, 16 * R);
+  const AcWork w = ac_work<T, HD>(p, gr, 16 * R);
   if (w.j0 >= w.j1) {                // nothing of this sequence in this split
     pdl_wait();
     return;
@@ -328,9 +334,10 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
       // The tensor core truncates when it adds to its accumulator, so a long chain
       // drifts by half a step of the sum per product.  Chains are kept to four
       // products and added up in fp32 (rounded): 1.6e-6 -> 5e-7 of the result.
-      float lo[2][4];                // hi lo and lo hi: small, one chain
+      // Six accumulators take turns, so that none waits for its last product.
+      float hl[2][4], lh[2][4];      // hi lo and lo hi: small, one chain each
 #pragma unroll
-      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] = lo[a >> 2][a & 3] = 0.f;
+      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] = hl[a >> 2][a & 3] = lh[a >> 2][a & 3] = 0.f;
 #pragma unroll
       for (int cg = 0; cg < HD / 32; ++cg) {
         float c[2][4];
@@ -349,25 +356,24 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
           const float kv[2][2][2] = {{{k0.x, k0.y}, {k1.x, k1.y}}, {{k0.z, k0.w}, {k1.z, k1.w}}};
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
-            uint32_t ah[4], al[4];
+            uint32_t ah[4], al[4], bh[2][2], bl[2][2];
 #pragma unroll
             for (int x = 0; x < 4; ++x) split_tf32(qv[st][x], ah[x], al[x]);
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              uint32_t h0, h1, l0, l1;
-              split_tf32(kv[st][n][0], h0, l0);
-              split_tf32(kv[st][n][1], h1, l1);
-              mma_tf32(c[n], ah, h0, h1);
-              mma_tf32(lo[n], ah, l0, l1);
-              mma_tf32(lo[n], al, h0, h1);
-            }
+            for (int x = 0; x < 4; ++x) split_tf32(kv[st][x >> 1][x & 1], bh[x >> 1][x & 1], bl[x >> 1][x & 1]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) mma_tf32(c[n], ah, bh[n][0], bh[n][1]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) mma_tf32(hl[n], ah, bl[n][0], bl[n][1]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) mma_tf32(lh[n], al, bh[n][0], bh[n][1]);
           }
         }
 #pragma unroll
         for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] += c[a >> 2][a & 3];
       }
 #pragma unroll
-      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] += lo[a >> 2][a & 3];
+      for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] += hl[a >> 2][a & 3] + lh[a >> 2][a & 3];
     }
     // ---- running softmax ----
     float mx_lo = -INFINITY, mx_hi = -INFINITY;
@@ -451,15 +457,18 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
           const float4 v0 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4, 8 * cg + g));
           const float4 v1 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4 + 1, 8 * cg + g));
           const float a[4] = {v0.x, v0.y, v0.z, v0.w}, b[4] = {v1.x, v1.y, v1.z, v1.w};
+          uint32_t h[4][2], lo[4][2];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            uint32_t h0, h1, l0, l1;
-            split_tf32(a[x], h0, l0);
-            split_tf32(b[x], h1, l1);
-            mma_tf32(c[x], ph[n], l0, l1);
-            mma_tf32(c[x], pl[n], h0, h1);
-            mma_tf32(c[x], ph[n], h0, h1);
+            split_tf32(a[x], h[x][0], lo[x][0]);
+            split_tf32(b[x], h[x][1], lo[x][1]);
           }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mma_tf32(c[x], ph[n], lo[x][0], lo[x][1]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mma_tf32(c[x], pl[n], h[x][0], h[x][1]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) mma_tf32(c[x], ph[n], h[x][0], h[x][1]);
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x) o[4 * cg + (x >> 2)][x & 3] += c[x >> 2][x & 3];
@@ -536,8 +545,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
 
 // ---- fp32, few rows -------------------------------------------------------------
 // A warp takes RN query rows and tiles of 32 / RN keys.  Lane l holds the dims
-// 4 l .. 4 l + 3 (and 128 + those; 2 l, 2 l + 1 at head_dim 64) of the rows, and
-// loads those of each key straight into registers: whole rows, coalesced, with no
+// 4 l .. 4 l + 3 (and 128 + those at head_dim 256) of the rows, and loads those of each key straight into registers: whole rows, coalesced, with no
 // shared memory between.  The 32 partial products of a tile (keys x rows) are
 // summed over the lanes by halving: at each of five steps a lane passes on half of
 // its values and keeps the other half, so 31 exchanges leave lane l with the logit
@@ -547,7 +555,6 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
 // would spend three tf32 products of 16 rows each on it (fp32, two sequences of
 // 65536 rows, four query rows: 253 us there).
 constexpr int AV_WARPS = 4;
-constexpr int AV_MAX_ROWS = 16;
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   unsigned long long d;
@@ -558,31 +565,28 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 template <int HD, int RN>
-__global__ void __launch_bounds__(AV_WARPS * 32, 2) ac_vec_kernel(const __grid_constant__ AcParams p, int prefix_part, int row_tiles) {
+__global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kernel(const __grid_constant__ AcParams p, AcGrid gr) {
   constexpr int KT = 32 / RN;                      // keys of a tile
   constexpr int D2 = HD / 64;                      // float2 of a lane
   __shared__ float merge[AV_WARPS][RN][HD];
   __shared__ float2 s_ml[AV_WARPS][RN];
+  __shared__ float s_q[RN][HD];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
-  const AcWork w = ac_work<float, HD>(p, prefix_part, row_tiles, RN);
+  const AcWork w = ac_work<float, HD>(p, gr, RN);
   if (w.j0 >= w.j1) {
     pdl_wait();
     return;
   }
   const long long key_stride = (long long)p.nkv * HD;
   // dims of float2 i of this lane: pairs (0, 1) and (2, 3) are one 16-byte access
-  auto dim = [&](int i) { return HD == 64 ? 2 * lane : 128 * (i >> 1) + 4 * lane + 2 * (i & 1); };
+  auto dim = [&](int i) { return 128 * (i >> 1) + 4 * lane + 2 * (i & 1); };
   auto load = [&](const float* src, bool ok, float2 (&x)[D2]) {
-    if constexpr (HD == 64) {
-      x[0] = ok ? *(const float2*)(src + 2 * lane) : make_float2(0.f, 0.f);
-    } else {
 #pragma unroll
-      for (int i = 0; i < D2; i += 2) {
-        const float4 y = ok ? *(const float4*)(src + dim(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[i] = make_float2(y.x, y.y);
-        x[i + 1] = make_float2(y.z, y.w);
-      }
+    for (int i = 0; i < D2; i += 2) {
+      const float4 y = ok ? *(const float4*)(src + dim(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[i] = make_float2(y.x, y.y);
+      x[i + 1] = make_float2(y.z, y.w);
     }
   };
   auto load_tile = [&](const uint8_t* base, int key0, float2 (&x)[KT][D2]) {
@@ -595,15 +599,24 @@ __global__ void __launch_bounds__(AV_WARPS * 32, 2) ac_vec_kernel(const __grid_c
   load_tile(w.k, key0, kx);
   load_tile(w.v, key0, vx);
 
-  float2 q[RN][D2], o[RN][D2];
+  // Q in shared memory: at head_dim 128 its registers are worth more as a third
+  // CTA per SM (four sequences of 30000 rows: 82 -> 74 us)
+  for (int id = tid; id < RN * (HD / 4); id += AV_WARPS * 32) {
+    const int r = id / (HD / 4), c = id % (HD / 4);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (w.row0 + r < w.nrows) {
+      int b, t, h;
+      ac_row(p, w, w.row0 + r, b, t, h);
+      x = *(const float4*)((const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD + 4 * c);
+    }
+    *(float4*)&s_q[r][4 * c] = x;
+  }
+  __syncthreads();
+  float2 o[RN][D2];
 #pragma unroll
-  for (int r = 0; r < RN; ++r) {
-    int b, t, h;
-    ac_row(p, w, min(w.row0 + r, w.nrows - 1), b, t, h);
-    load((const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD, w.row0 + r < w.nrows, q[r]);
+  for (int r = 0; r < RN; ++r)
 #pragma unroll
     for (int i = 0; i < D2; ++i) o[r][i] = make_float2(0.f, 0.f);
-  }
   // this lane's key and row of a tile
   const int my_key = lane / RN, my_row = lane % RN;
   int lim = 0;
@@ -620,14 +633,17 @@ __global__ void __launch_bounds__(AV_WARPS * 32, 2) ac_vec_kernel(const __grid_c
     // ---- S = Q K^T ----
     float s[32];
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
+    for (int r = 0; r < RN; ++r) {
+      float2 q[D2];
+      load(s_q[r], true, q);
 #pragma unroll
-      for (int r = 0; r < RN; ++r) {
+      for (int k = 0; k < KT; ++k) {
         float2 a = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < D2; ++i) a = fma2(kx[k][i], q[r][i], a);
+        for (int i = 0; i < D2; ++i) a = fma2(kx[k][i], q[i], a);
         s[k * RN + r] = a.x + a.y;
       }
+    }
     load_tile(w.k, key0 + AV_WARPS * KT, kx);
 #pragma unroll
     for (int st = 16; st >= 1; st >>= 1) {
@@ -850,17 +866,22 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
 
 // ---- host ---------------------------------------------------------------------
 struct AcPlan {
-  bool p_tc;                      // prefix part on tcgen05
+  bool p_tc;                      // prefix part on tcgen05 (ap_rows() rows per CTA)
   int p_r, o_r;                   // rows per CTA of the two parts: 16, 32, 64 (ac_part_kernel), 4, 8 (ac_vec_kernel)
-  int p_tiles, o_tiles;           // row tiles
+  int p_tiles;                    // row tiles of the prefix part
   long long rows;                 // query rows over all heads
   size_t off_ml, off_logits, bytes;
 };
 
-// Rows per CTA for a part with `rows` query rows per KV head: fp32 with few rows
-// goes to ac_vec_kernel in tiles of 4 or 8
-int ac_row_class(int type, long long rows) {
-  if (type == INFERNO_F32 && rows <= AV_MAX_ROWS) return rows <= 4 ? 4 : 8;
+// Rows per CTA for a part with `rows` query rows per KV head and `len` keys.  fp32
+// with few rows goes to ac_vec_kernel in tiles of 4 or 8, where the tensor cores'
+// three products cost more than the lanes' sums: head_dim 256 up to 8 rows (two
+// sequences of 30000: 115 us against 142), or 16 over few keys, which end sooner
+// there (prefix of 500: 11 us against 18; 30000: 178 against 152); 128 up to 4
+// (four of 30000: 74 against 94; 8 rows: 105 against 98); not 64 (4 rows: 69
+// against 58).
+int ac_row_class(int type, int hd, long long rows, int len) {
+  if (type == INFERNO_F32 && rows <= (hd == 256 ? (len <= 4096 ? 16 : 8) : hd == 128 ? 4 : 0)) return rows <= 4 ? 4 : 8;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
@@ -917,11 +938,18 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   p->group = a->n_heads / a->n_kv_heads;
   p->prefix_len = a->prefix_len;
   p->max_len = a->max_len;
+  p->by_seq = FastDiv((uint32_t)(a->n_tokens * p->group));
+  p->by_group = FastDiv((uint32_t)p->group);
   const long long own = (long long)a->n_tokens * p->group, pre = own * a->batch;
   pl.rows = pre * a->n_kv_heads;
-  pl.o_r = ac_row_class(a->type, own);
-  pl.p_r = ac_row_class(a->type, pre);
-  pl.o_tiles = (int)((own + pl.o_r - 1) / pl.o_r);
+  pl.o_r = ac_row_class(a->type, a->head_dim, own, a->max_len);
+  pl.p_r = ac_row_class(a->type, a->head_dim, pre, a->prefix_len);
+  // both parts in one launch where the own part is small beside the prefix and
+  // can take the prefix part's kernel: a launch costs more than idle rows then
+  if (a->prefix_len && a->max_len && pl.p_r > pl.o_r && (pl.p_r <= 8 || pl.o_r >= 16) && !ac_prefix_tc(a->type, pre) &&
+      (long long)a->max_len * a->batch <= a->prefix_len)
+    pl.o_r = pl.p_r;
+  const int o_tiles = (int)((own + pl.o_r - 1) / pl.o_r);
   pl.p_tiles = (int)((pre + pl.p_r - 1) / pl.p_r);
   pl.p_tc = ac_prefix_tc(a->type, pre);
   if (pl.p_tc) {
@@ -935,7 +963,7 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   } else {
     ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, &p->p_splits, &p->p_split_len);
   }
-  ac_split((long long)pl.o_tiles * a->n_kv_heads * a->batch, a->max_len, &p->o_splits, &p->o_split_len);
+  ac_split((long long)o_tiles * a->n_kv_heads * a->batch, a->max_len, &p->o_splits, &p->o_split_len);
   p->n_splits = p->p_splits + p->o_splits;
   p->logit_stride = a->scores ? ((long long)a->max_len + 15) / 16 * 16 : 0;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
@@ -965,37 +993,50 @@ cudaError_t ac_launch(void (*kernel)(Args...), long long blocks, int threads, si
 }
 
 template <typename T, int HD, int R>
-cudaError_t ac_launch_part(const AcParams& p, int prefix_part, int tiles, long long blocks, bool beside, cudaStream_t st) {
+cudaError_t ac_launch_part(const AcParams& p, AcGrid gr, long long blocks, bool beside, cudaStream_t st) {
   using G = AcGeo<T, HD, R>;
   static DeviceOnce once;
   cudaError_t e = once.run([] {
     return cudaFuncSetAttribute(ac_part_kernel<T, HD, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
   });
   if (e != cudaSuccess) return e;
-  return ac_launch(ac_part_kernel<T, HD, R>, blocks, G::THREADS, G::SMEM, st, beside, p, prefix_part, tiles);
+  return ac_launch(ac_part_kernel<T, HD, R>, blocks, G::THREADS, G::SMEM, st, beside, p, gr);
 }
+// one kernel over the prefix part, the own part or both, r rows per CTA
 template <typename T, int HD>
-cudaError_t ac_part(const AcParams& p, int r, int prefix_part, int tiles, bool beside, cudaStream_t st) {
-  const long long blocks = (long long)tiles * p.nkv * (prefix_part ? p.p_splits : (long long)p.o_splits * p.batch);
-  if constexpr (AcType<T>::F32) {
-    if (r == 4) return ac_launch(ac_vec_kernel<HD, 4>, blocks, AV_WARPS * 32, 0, st, beside, p, prefix_part, tiles);
-    if (r == 8) return ac_launch(ac_vec_kernel<HD, 8>, blocks, AV_WARPS * 32, 0, st, beside, p, prefix_part, tiles);
+cudaError_t ac_part(const AcParams& p, const AcPlan& pl, int r, bool prefix, bool own, bool beside, cudaStream_t st) {
+  const long long pt = ((long long)p.batch * p.n_tok * p.group + r - 1) / r, ot = ((long long)p.n_tok * p.group + r - 1) / r;
+  const long long pb = prefix ? pt * p.nkv * p.p_splits : 0;
+  const long long blocks = pb + (own ? ot * p.nkv * p.o_splits * p.batch : 0);
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  const AcGrid gr{(int)pb, (int)pt, (int)ot};
+  if constexpr (AcType<T>::F32 && HD >= 128) {
+    if (r == 4) return ac_launch(ac_vec_kernel<HD, 4>, blocks, AV_WARPS * 32, 0, st, beside, p, gr);
   }
-  return r == 16   ? ac_launch_part<T, HD, 1>(p, prefix_part, tiles, blocks, beside, st)
-         : r == 32 ? ac_launch_part<T, HD, 2>(p, prefix_part, tiles, blocks, beside, st)
-                   : ac_launch_part<T, HD, 4>(p, prefix_part, tiles, blocks, beside, st);
+  if constexpr (AcType<T>::F32 && HD == 256) {
+    if (r == 8) return ac_launch(ac_vec_kernel<HD, 8>, blocks, AV_WARPS * 32, 0, st, beside, p, gr);
+  }
+  return r == 16   ? ac_launch_part<T, HD, 1>(p, gr, blocks, beside, st)
+         : r == 32 ? ac_launch_part<T, HD, 2>(p, gr, blocks, beside, st)
+                   : ac_launch_part<T, HD, 4>(p, gr, blocks, beside, st);
 }
 template <typename T, int HD>
 cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   bool any = pl.p_tc && p.p_splits;    // a kernel of this call is in flight
-  if (p.p_splits && !pl.p_tc) {
-    e = ac_part<T, HD>(p, pl.p_r, 1, pl.p_tiles, false, st);
+  const bool prefix = p.p_splits && !pl.p_tc, own = p.o_splits > 0;
+  if (prefix && own && pl.p_r == pl.o_r) {
+    e = ac_part<T, HD>(p, pl, pl.p_r, true, true, false, st);
     any = true;
-  }
-  if (e == cudaSuccess && p.o_splits) {
-    e = ac_part<T, HD>(p, pl.o_r, 0, pl.o_tiles, any, st);
-    any = true;
+  } else {
+    if (prefix) {
+      e = ac_part<T, HD>(p, pl, pl.p_r, true, false, false, st);
+      any = true;
+    }
+    if (e == cudaSuccess && own) {
+      e = ac_part<T, HD>(p, pl, pl.o_r, false, true, any, st);
+      any = true;
+    }
   }
   if (e != cudaSuccess) return e;
   // four warps per row when it has more splits than one warp has in flight

@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include "longctx.h"
 
 namespace inf {
 
@@ -18,6 +19,7 @@ struct AcParams {
   float* scores;
   long long q_stride, out_stride, seq_stride, score_stride;   // elements
   int batch, n_tok, nh, nkv, group, prefix_len, max_len;
+  FastDiv by_seq, by_group;      // a sequence's rows of one KV head, n_tok * group; group
   float scale_log2;              // scale * log2(e)
   // splits: prefix splits come first, then own ones; split s of a part covers
   // its keys [s * len, (s + 1) * len)

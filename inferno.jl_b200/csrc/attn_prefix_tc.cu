@@ -107,6 +107,13 @@ __device__ __forceinline__ uint32_t ap_pack2(float a, float b) {
   }
 }
 
+// row r of a KV head's rows -> token row (b * n_tok + t) and query head
+__device__ __forceinline__ void ap_row(const AcParams& p, int kvh, int r, int& tok, int& h) {
+  const int b = (int)p.by_seq.div(r), tg = r - b * (int)p.by_seq.d, t = (int)p.by_group.div(tg);
+  tok = b * p.n_tok + t;
+  h = kvh * p.group + tg - t * p.group;
+}
+
 struct alignas(64) ApMaps {
   CUtensorMap k, v;
 };
@@ -244,12 +251,12 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
     // ================= softmax: one row per thread =================
     // a thread's 16-byte column is the same in all its rows; all copies in flight
     constexpr int CH = HD / 8, STEP = AP_M / CH;
-    const int c = tid % CH, per_b = p.n_tok * p.group;
+    const int c = tid % CH;
 #pragma unroll 8
     for (int r = tid / CH; r < AP_M; r += STEP) {
-      const int rr = min(row0 + r, nrows - 1), b = rr / per_b, tg = rr - b * per_b, t = tg / p.group;
-      const T* src = (const T*)p.q + (long long)(b * p.n_tok + t) * p.q_stride +
-                     (long long)(kvh * p.group + tg - t * p.group) * HD + c * 8;
+      int tok, h;
+      ap_row(p, kvh, min(row0 + r, nrows - 1), tok, h);
+      const T* src = (const T*)p.q + (long long)tok * p.q_stride + (long long)h * HD + c * 8;
       cp_async16(smem_u32(s_q) + (c >> 3) * AP_M * 128 + sw128_off(r, c & 7), src, row0 + r < nrows);
     }
     cp_commit();
@@ -355,13 +362,13 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       // shared memory (the K ring, idle now; 36 floats apart, so that neither side
       // of the turn has two lanes of a phase on one bank), eight lanes per row
       float* turn = (float*)s_k + warp * 32 * 36;
-      const int per_b = p.n_tok * p.group;
       long long at[8];                                  // this lane's rows lane / 8 + 4 i
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = row0 + warp * 32 + i * 4 + (lane >> 3);
-        const int b = r / per_b, tg = r - b * per_b, t = tg / p.group;
-        at[i] = r < nrows ? ((long long)(b * p.n_tok + t) * p.nh + kvh * p.group + (tg - t * p.group)) * p.n_splits + split : -1;
+        int tok, h;
+        ap_row(p, kvh, r, tok, h);
+        at[i] = r < nrows ? ((long long)tok * p.nh + h) * p.n_splits + split : -1;
       }
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
@@ -379,8 +386,9 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       }
       const int r = row0 + tid;
       if (r < nrows) {
-        const int b = r / per_b, tg = r - b * per_b, t = tg / p.group;
-        p.part_ml[((long long)(b * p.n_tok + t) * p.nh + kvh * p.group + (tg - t * p.group)) * p.n_splits + split] = make_float2(m, l);
+        int tok, h;
+        ap_row(p, kvh, r, tok, h);
+        p.part_ml[((long long)tok * p.nh + h) * p.n_splits + split] = make_float2(m, l);
       }
     }
   }

@@ -421,13 +421,16 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.max_moves = evict_max_moves(e);
   p.lists = (int*)workspace;
   if (e->lens_out == e->lens) p.lens_out = nullptr;
-  // CTAs per (sequence, KV head): up to 8 while a CTA keeps 512 rows (fewer do not
-  // pay for the wider barriers) and all CTAs run at once, two per SM
+  // CTAs per (sequence, KV head), up to 8 and while all run at once, two per SM: one
+  // per 4096 rows to rank (fewer do not pay for the cluster's barriers, of which one
+  // CTA has none) or per 256 KB to move
   const int n = e->batch * e->n_kv_heads;
   int dev = 0;
   INF_CUDA_TRY(cudaGetDevice(&dev));
   int nc = 1;
-  while (nc < EV_MAX_CLUSTER && e->max_len >= nc * 2 * 512 && n * nc * 2 <= 2 * num_sms(dev)) nc *= 2;
+  while (nc < EV_MAX_CLUSTER && n * nc * 2 <= 2 * num_sms(dev) &&
+         (e->max_len >= nc * 2 * 4096 || 4ll * p.max_moves * p.head_bytes >= nc * 2 * (256ll << 10)))
+    nc *= 2;
   auto smem_of = [&](int ctas, bool cached) {
     const long long words = ((e->max_len + 31) / 32 + ctas - 1) / ctas;
     return words * 4 * (5 + (cached ? 32 : 0));

@@ -7,6 +7,18 @@
 
 namespace inf {
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994)
+struct FastDiv {
+  uint32_t d, mul, shift;
+  __host__ FastDiv(uint32_t div = 1) : d(div) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 // bytes of an element of the operators' types, 0 for any other type
 inline int longctx_type_size(int type) {
   return type == INFERNO_F32 ? 4 : type == INFERNO_F16 || type == INFERNO_BF16 ? 2 : 0;

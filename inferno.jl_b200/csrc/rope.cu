@@ -30,18 +30,6 @@ namespace inf {
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_MAX_PAIRS = 256;
 
-// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, "Division by
-// invariant integers using multiplication", 1994)
-struct FastDiv {
-  uint32_t d, mul, shift;
-  __host__ FastDiv(uint32_t div = 1) : d(div) {
-    shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-
 struct RopeParams {
   const void *q, *k, *v;
   void *qo, *ko, *vo;
