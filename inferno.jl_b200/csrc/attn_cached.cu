@@ -241,6 +241,17 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
     }
     cp_commit();
   };
+  if constexpr (F32) {       // Q ahead of the ring, part of its first copy group
+    constexpr int CH = ROW / 16;
+#pragma unroll 4
+    for (int id = tid; id < 16 * R * CH; id += G::THREADS) {
+      const int r = id / CH, c = id % CH;
+      int b, t, h;
+      ac_row(p, w, min(w.row0 + r, w.nrows - 1), b, t, h);
+      cp_async16(tile_addr<ROW>(s_q, r, c), (const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD + 4 * c,
+                 w.row0 + r < w.nrows);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i) issue(i);
 
@@ -271,15 +282,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
         qf[k][3] = q_hi ? *(const uint32_t*)(q_hi + d + 8) : 0u;
       }
     } else {
-      for (int id = tid; id < 16 * R * (ROW / 16); id += G::THREADS) {
-        const int r = id / (ROW / 16), c = id % (ROW / 16);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (w.row0 + r < w.nrows) {
-          ac_row(p, w, w.row0 + r, b, t, h);
-          x = *(const float4*)((const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD + 4 * c);
-        }
-        *(float4*)(smem + (tile_addr<ROW>(0, r, c))) = x;
-      }
+      cp_wait<SLOTS - 2>();
       __syncthreads();
     }
   }
@@ -514,6 +517,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
   }
   __syncthreads();
   const int live = min(16 * R, w.nrows - w.row0);
+#pragma unroll 4
   for (int id = tid; id < live * (HD / 4); id += G::THREADS) {
     const int r = id / (HD / 4), c = id % (HD / 4), tile = r >> 4, rr = r & 15;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
