@@ -183,7 +183,7 @@ int inferno_gdn_chunked(int T, int n_heads, int dk, int dv, const float* q, cons
  * sequence.  `type` is INFERNO_F32, INFERNO_F16 or INFERNO_BF16 and holds for
  * q, k, v, caches and outputs alike; sums, softmax statistics and gathered
  * weights are fp32.  Pointers are device pointers of the current device;
- * struct_size must be sizeof of the struct.  The calls are asynchronous on
+ * struct_size is sizeof of the struct (0 is taken for that).  The calls are asynchronous on
  * `stream`, allocate nothing, can be captured into a graph, and read lengths,
  * positions and slots on the device only.  A workspace holds nothing between
  * calls and needs no initialisation; calls that may run at the same time (two

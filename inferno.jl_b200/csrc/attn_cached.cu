@@ -914,7 +914,7 @@ bool ac_prefix_tc(int type, long long rows) { return type != INFERNO_F32 && rows
 
 int ac_check(const InfernoAttention* a) {
   if (!a) return set_error(INFERNO_EINVAL, "attention_cached: null parameters");
-  if (a->struct_size != (int)sizeof(InfernoAttention))
+  if (a->struct_size && a->struct_size != (int)sizeof(InfernoAttention))
     return set_error(INFERNO_EINVAL, "attention_cached: struct_size %d, expected %d", a->struct_size,
                      (int)sizeof(InfernoAttention));
   if (!longctx_type_size(a->type))

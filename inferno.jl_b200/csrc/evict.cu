@@ -58,7 +58,7 @@ struct EvShared {
   int4 border;                        // ties before / behind the budget, other rows to leave before it / to keep behind it
   int always;                         // rows kept always
   // the CTA's own
-  int total[EV_BINS];                 // counts over the cluster
+  alignas(16) int total[EV_BINS];     // counts over the cluster
   int warp_sums[2][EV_WARPS];
 };
 
@@ -113,6 +113,10 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
     }
     return;
   }
+  auto sync_all = [&] {
+    if (nc == 1) __syncthreads();
+    else cluster.sync();
+  };
   // this CTA's rows [j0, j0 + n), in words of 32
   const int words_all = (len + 31) >> 5, wpc = (words_all + nc - 1) / nc;
   const int j0 = min(c * wpc, words_all) * 32, n = min(len - j0, wpc * 32), nw = (n + 31) >> 5;
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
           atomicAdd(&sh.hist[buf][(k >> shift) & 255], 1);
       }
     }
-    cluster.sync();
+    sync_all();
     if (shift == 24 && !recount) {
       int al = lane < nc ? *cluster.map_shared_rank(&sh.always, lane) : 0;
       al = __reduce_add_sync(0xffffffffu, al);
@@ -187,7 +191,11 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
     // largest key (need 0: no row of this class, any digit does)
     int cnt[8], mine = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mine += cnt[i] = sh.total[8 * lane + i];
+    for (int i = 0; i < 8; i += 4) {
+      const int4 x = *(const int4*)&sh.total[8 * lane + i];
+      cnt[i] = x.x, cnt[i + 1] = x.y, cnt[i + 2] = x.z, cnt[i + 3] = x.w;
+      mine += x.x + x.y + x.z + x.w;
+    }
     int above = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -239,7 +247,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   ev_scan(sh, ties, ties_front, sum, sum_front);
   ev_scan(sh, leave, stay, sum_leave, sum_stay);
   if (t == 0) sh.border = make_int4(sum_front, sum - sum_front, sum_leave, sum_stay);
-  cluster.sync();
+  sync_all();
   // lane r: CTA r's part.  Its ties are kept as far as `need` reaches after those
   // of the CTAs before it, the ones before the budget first
   int holes, srcs, moves;
@@ -281,49 +289,64 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   int* hole_list = p.lists + (long long)bh * 2 * p.max_moves;
   int* src_list = hole_list + p.max_moves;
   const uint32_t lt = (1u << lane) - 1;
-  for (int w = warp; w < nw; w += EV_WARPS) {
-    const int i = w * 32 + lane, j = j0 + i;
-    const uint32_t k = keep[w];
-    const bool kept = (k >> lane) & 1, front = j < p.budget;
-    const uint32_t m_h = __ballot_sync(0xffffffffu, i < n && front && !kept);
-    const uint32_t m_s = __ballot_sync(0xffffffffu, !front && kept);
-    if ((m_h >> lane) & 1) hole_list[base_h[w] + __popc(m_h & lt)] = j;
-    if ((m_s >> lane) & 1) src_list[base_s[w] + __popc(m_s & lt)] = j;
-    if (front && kept) {
-      if (so != sc) so[j] = sc[j];
-      if (po != ps) po[j] = ps[j];
+  const bool copy = so != sc || po != ps;
+  for (int w0 = warp; w0 < nw; w0 += 4 * EV_WARPS) {
+    float x[4];
+    int at[4];
+    if (copy) {                               // four words' loads in flight
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int w = w0 + u * EV_WARPS, i = w * 32 + lane;
+        const bool stays = w < nw && j0 + i < p.budget && ((keep[min(w, nw - 1)] >> lane) & 1);
+        x[u] = stays ? sc[j0 + i] : 0.f;
+        at[u] = stays ? ps[j0 + i] : 0;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int w = w0 + u * EV_WARPS, i = w * 32 + lane, j = j0 + i;
+      if (w >= nw) break;
+      const bool kept = (keep[w] >> lane) & 1, front = j < p.budget;
+      const uint32_t m_h = __ballot_sync(0xffffffffu, i < n && front && !kept);
+      const uint32_t m_s = __ballot_sync(0xffffffffu, !front && kept);
+      if ((m_h >> lane) & 1) hole_list[base_h[w] + __popc(m_h & lt)] = j;
+      if ((m_s >> lane) & 1) src_list[base_s[w] + __popc(m_s & lt)] = j;
+      if (copy && front && kept) so[j] = x[u], po[j] = at[u];
     }
   }
-  cluster.sync();                             // lists complete; also the last read of a peer's shared memory
+  sync_all();                             // lists complete; also the last read of a peer's shared memory
 
   // ---- move ---------------------------------------------------------------------------
+  const int vecs = p.head_bytes / 16;         // 16-byte pieces of a K row; as many of the V row
+  uint8_t* kb = p.kc + b * p.seq_bytes + (long long)h * p.head_bytes;
+  uint8_t* vb = p.vc + b * p.seq_bytes + (long long)h * p.head_bytes;
+  const int iters = (2 * vecs + 31) / 32, stride = nc * EV_WARPS, first = c * EV_WARPS + warp;
+  const int mine = moves > first ? (moves - first + stride - 1) / stride : 0;
+  constexpr int U = 6;                        // pieces in flight per lane
+  int m = 0, it = 0;                          // move and piece of the next unit
+  for (int u0 = 0; u0 < mine * iters; u0 += U) {
+    uint4 x[U];
+    int to[U], piece[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      piece[u] = it * 32 + lane;
+      to[u] = -1;
+      if (m < mine && piece[u] < 2 * vecs) {
+        const int at = first + m * stride;
+        const uint8_t* base = piece[u] < vecs ? kb + piece[u] * 16 : vb + (piece[u] - vecs) * 16;
+        to[u] = hole_list[at];
+        x[u] = *(const uint4*)(base + src_list[at] * p.row_bytes);
+      }
+      if (++it == iters) it = 0, ++m;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (to[u] >= 0) *(uint4*)((piece[u] < vecs ? kb + piece[u] * 16 : vb + (piece[u] - vecs) * 16) + to[u] * p.row_bytes) = x[u];
+  }
   for (int i = c * EV_THREADS + t; i < moves; i += nc * EV_THREADS) {
     const int from = src_list[i], to = hole_list[i];
     so[to] = sc[from];
     po[to] = ps[from];
-  }
-  const int vecs = p.head_bytes / 16;         // 16-byte pieces of a K row; as many of the V row
-  uint8_t* kb = p.kc + b * p.seq_bytes + (long long)h * p.head_bytes;
-  uint8_t* vb = p.vc + b * p.seq_bytes + (long long)h * p.head_bytes;
-  const int iters = (2 * vecs + 31) / 32, stride = nc * EV_WARPS;
-  const int mine = moves > c * EV_WARPS + warp ? (moves - (c * EV_WARPS + warp) + stride - 1) / stride : 0;
-  constexpr int U = 4;                        // pieces in flight per lane
-  for (int u0 = 0; u0 < mine * iters; u0 += U) {
-    uint4 x[U];
-    uint8_t* dst[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      dst[u] = nullptr;
-      const int unit = u0 + u, m = unit / iters, piece = (unit - m * iters) * 32 + lane;
-      if (m >= mine || piece >= 2 * vecs) continue;
-      const int at = c * EV_WARPS + warp + m * stride;
-      uint8_t* base = piece < vecs ? kb + piece * 16 : vb + (piece - vecs) * 16;
-      dst[u] = base + hole_list[at] * p.row_bytes;
-      x[u] = *(const uint4*)(base + src_list[at] * p.row_bytes);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (dst[u]) *(uint4*)dst[u] = x[u];
   }
 }
 
@@ -337,7 +360,7 @@ namespace {
 
 int evict_check(const InfernoEvict* e) {
   if (!e) return set_error(INFERNO_EINVAL, "cache_evict: null parameters");
-  if (e->struct_size != (int)sizeof(InfernoEvict))
+  if (e->struct_size && e->struct_size != (int)sizeof(InfernoEvict))
     return set_error(INFERNO_EINVAL, "cache_evict: struct_size %d, expected %d", e->struct_size,
                      (int)sizeof(InfernoEvict));
   const int es = longctx_type_size(e->type);
@@ -422,14 +445,14 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.lists = (int*)workspace;
   if (e->lens_out == e->lens) p.lens_out = nullptr;
   // CTAs per (sequence, KV head), up to 8 and while all run at once, two per SM: one
-  // per 4096 rows to rank (fewer do not pay for the cluster's barriers, of which one
-  // CTA has none) or per 256 KB to move
+  // per 1024 rows to rank (4160 rows in 32 heads: 17.7 us with four, 20.6 with one,
+  // which waits for itself instead of the others) or per 256 KB to move
   const int n = e->batch * e->n_kv_heads;
   int dev = 0;
   INF_CUDA_TRY(cudaGetDevice(&dev));
   int nc = 1;
   while (nc < EV_MAX_CLUSTER && n * nc * 2 <= 2 * num_sms(dev) &&
-         (e->max_len >= nc * 2 * 4096 || 4ll * p.max_moves * p.head_bytes >= nc * 2 * (256ll << 10)))
+         (e->max_len >= nc * 2 * 1024 || 4ll * p.max_moves * p.head_bytes >= nc * 2 * (256ll << 10)))
     nc *= 2;
   auto smem_of = [&](int ctas, bool cached) {
     const long long words = ((e->max_len + 31) / 32 + ctas - 1) / ctas;

@@ -256,7 +256,7 @@ using namespace inf;
 
 extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
   if (!r) return set_error(INFERNO_EINVAL, "rope: null parameters");
-  if (r->struct_size != (int)sizeof(InfernoRope))
+  if (r->struct_size && r->struct_size != (int)sizeof(InfernoRope))
     return set_error(INFERNO_EINVAL, "rope: struct_size %d, expected %d", r->struct_size, (int)sizeof(InfernoRope));
   const int es = longctx_type_size(r->type);
   if (!es) return set_error(INFERNO_EINVAL, "rope: type %d is not F32, F16 or BF16", r->type);

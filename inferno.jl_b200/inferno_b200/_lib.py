@@ -38,25 +38,12 @@ class InfernoSampling(C.Structure):
                 ("repetition_penalty", C.c_float), ("presence_penalty", C.c_float), ("seed", C.c_uint64)]
 
 
-class _Sized(C.Structure):
-    """A parameter struct whose struct_size is filled in."""
-
-    def __init__(self, **kw):
-        C.Structure.__init__(self, self._size, **kw)      # struct_size is the first field
-
-
-def _sized(cls):
-    cls._size = C.sizeof(cls)
-    return cls
-
-
 def _fields(kind, names):
     return [(n, kind) for n in names.split()]
 
 
-@_sized
-class InfernoRope(_Sized):
-    """include/inferno_b200.h InfernoRope (rotary positions with cache append)."""
+class InfernoRope(C.Structure):
+    """include/inferno_b200.h InfernoRope (rotary positions with cache append); struct_size may stay 0."""
     _fields_ = (_fields(C.c_int32, "struct_size type n_tokens n_heads n_kv_heads head_dim rope_dim layout scaling "
                                    "inverse orig_ctx n_rows")
                 + _fields(C.c_float, "theta factor beta_fast beta_slow mscale")
@@ -64,16 +51,14 @@ class InfernoRope(_Sized):
                 + _fields(C.c_int64, "q_stride k_stride v_stride q_out_stride k_out_stride v_out_stride"))
 
 
-@_sized
-class InfernoAttention(_Sized):
+class InfernoAttention(C.Structure):
     """include/inferno_b200.h InfernoAttention (shared prefix + per-sequence caches)."""
     _fields_ = (_fields(C.c_int32, "struct_size type batch n_tokens n_heads n_kv_heads head_dim prefix_len max_len")
                 + _fields(C.c_float, "scale") + _fields(C.c_int64, "q_stride out_stride seq_stride score_stride")
                 + _fields(C.c_void_p, "q prefix_k prefix_v k_cache v_cache lens scores out"))
 
 
-@_sized
-class InfernoEvict(_Sized):
+class InfernoEvict(C.Structure):
     """include/inferno_b200.h InfernoEvict (cache eviction by gathered weight)."""
     _fields_ = (_fields(C.c_int32, "struct_size type batch n_kv_heads head_dim max_len budget n_sink n_recent reserved")
                 + _fields(C.c_int64, "seq_stride score_stride")
