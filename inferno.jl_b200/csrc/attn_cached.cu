@@ -52,13 +52,15 @@ template <typename T, int HD, int R>
 struct AcGeo {
   static constexpr int ROW = HD * (int)sizeof(T);              // bytes of a K / V row of one head
   static constexpr int ITEM = AC_KT * ROW;                     // bytes of a ring slot
-  static constexpr int QBYTES = AcType<T>::F32 ? 16 * R * ROW : 0;
+  // Q in registers; of fp32 above head_dim 64 they are too few, it stays in shared memory
+  static constexpr bool QS = AcType<T>::F32 && HD > 64;
+  static constexpr int QBYTES = QS ? 16 * R * ROW : 0;
   // two CTAs of four warps per SM, so that one streams while the other starts or
   // merges; one CTA of up to eight warps where the half SM does not hold three
   // slots per group (fp32 at head_dim 256)
   static constexpr int ML = 8 * 16 * 8;
   static constexpr bool TWO = (4 / R) * 3 * ITEM + QBYTES + ML <= AC_SMEM_HALF &&
-                              4 * 16 * HD * 4 + QBYTES + ML <= AC_SMEM_HALF;   // ring and merge buffer share their space
+                              4 * 16 * HD * 4 + ML <= AC_SMEM_HALF;   // the merge buffer takes the place of Q and ring
   static constexpr int CTAS = TWO ? 2 : 1;
   static constexpr int ROOM = (TWO ? AC_SMEM_HALF : AC_SMEM) - ML - QBYTES;
   static constexpr int NG0 = (TWO ? 4 : 8) / R;
@@ -69,7 +71,8 @@ struct AcGeo {
   static constexpr int SLOTS = MAXSLOTS > 6 ? 6 : MAXSLOTS;
   static constexpr int RING = NG * SLOTS * ITEM;
   static constexpr int MERGE = NW * 16 * HD * 4;
-  static constexpr int SMEM = QBYTES + (RING > MERGE ? RING : MERGE) + NW * 16 * 8;
+  static constexpr int BODY = QBYTES + RING > MERGE ? QBYTES + RING : MERGE;
+  static constexpr int SMEM = BODY + NW * 16 * 8;
   static_assert(SLOTS >= 3 && SMEM <= (TWO ? AC_SMEM_HALF : AC_SMEM), "shared memory");
 };
 
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
   const uint32_t s_q = smem_u32(smem);                            // fp32 only: [16 R][HD]
   uint8_t* ring_p = smem + G::QBYTES;
   const uint32_t ring = smem_u32(ring_p) + grp * SLOTS * ITEM;
-  float2* s_ml = (float2*)(ring_p + (G::RING > G::MERGE ? G::RING : G::MERGE));   // [NW][16]
+  float2* s_ml = (float2*)(smem + G::BODY);                      // [NW][16]
 
   // tiles of this group: grp, grp + NG, ...; item 2 i is K of its i-th tile, 2 i + 1 V
   const int ntiles = (w.j1 - w.j0 + AC_KT - 1) / AC_KT;
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
     }
     cp_commit();
   };
-  if constexpr (F32) {       // Q ahead of the ring, part of its first copy group
+  if constexpr (G::QS) {     // Q ahead of the ring, part of its first copy group
     constexpr int CH = ROW / 16;
 #pragma unroll 4
     for (int id = tid; id < 16 * R * CH; id += G::THREADS) {
@@ -255,8 +258,10 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i) issue(i);
 
-  // ---- Q: 16-bit types in registers as A fragments, fp32 in shared memory ----
+  // ---- Q: A fragments in registers (fp32: the float4 of each 16-byte column that
+  // S takes of the two rows), or in shared memory ----
   uint32_t qf[F32 ? 1 : HD / 16][4];
+  float4 qr[F32 && !G::QS ? HD / 16 : 1][2];
   const int r_lo = w.row0 + rt * 16 + g, r_hi = r_lo + 8;         // the two rows of this thread
   int lim_lo = 0, lim_hi = 0;                                     // keys they see
   {
@@ -281,9 +286,16 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
         qf[k][2] = q_lo ? *(const uint32_t*)(q_lo + d + 8) : 0u;
         qf[k][3] = q_hi ? *(const uint32_t*)(q_hi + d + 8) : 0u;
       }
-    } else {
+    } else if constexpr (G::QS) {
       cp_wait<SLOTS - 2>();
       __syncthreads();
+    } else {
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        const int d = 4 * (8 * (i >> 1) + 2 * t4 + (i & 1));
+        qr[i][0] = q_lo ? *(const float4*)(q_lo + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        qr[i][1] = q_hi ? *(const float4*)(q_hi + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
     }
   }
   float* lg_lo = nullptr;
@@ -313,11 +325,17 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
     else named_bar_sync(1 + grp, GT);
   };
 
+  const bool busy = w.row0 + rt * 16 < w.nrows;      // the warp has rows; else it only copies
   for (int i = 0; i < my_tiles; ++i) {
     const int key0 = w.j0 + (grp + i * G::NG) * AC_KT;
     // ---- S = Q K^T ----
     landed();
     issue(2 * i + SLOTS - 1);
+    if (!busy) {
+      landed();
+      issue(2 * i + 1 + SLOTS - 1);
+      continue;
+    }
     const uint32_t kt = ring + ((2 * i) % SLOTS) * ITEM;
     float s[2][4];
     if constexpr (!F32) {
@@ -351,8 +369,13 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
           // four consecutive dims per thread, used as the k indices t4 and t4 + 4
           // of two k steps, the same dims of Q and K
           const int ch = 8 * cg + 2 * t4 + e;
-          const float4 qa = lds_f4(tile_addr<ROW>(s_q, rt * 16 + g, ch));
-          const float4 qb = lds_f4(tile_addr<ROW>(s_q, rt * 16 + g + 8, ch));
+          float4 qa, qb;
+          if constexpr (G::QS) {
+            qa = lds_f4(tile_addr<ROW>(s_q, rt * 16 + g, ch));
+            qb = lds_f4(tile_addr<ROW>(s_q, rt * 16 + g + 8, ch));
+          } else {
+            qa = qr[2 * cg + e][0], qb = qr[2 * cg + e][1];
+          }
           const float4 k0 = lds_f4(tile_addr<ROW>(kt, g, ch));
           const float4 k1 = lds_f4(tile_addr<ROW>(kt, g + 8, ch));
           const float qv[2][4] = {{qa.x, qb.x, qa.y, qb.y}, {qa.z, qb.z, qa.w, qb.w}};
@@ -490,7 +513,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
     s_ml[warp * 16 + g + 8] = make_float2(m_hi, l_hi);
   }
   cp_wait<0>();
-  __syncthreads();                     // every group is done with its ring
+  __syncthreads();                     // every group is done with Q and its ring
   float M_lo = -INFINITY, M_hi = -INFINITY;
 #pragma unroll
   for (int x = 0; x < G::NG; ++x) {
@@ -498,7 +521,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
     M_hi = fmaxf(M_hi, s_ml[(x * R + rt) * 16 + g + 8].x);
   }
   const float f_lo = ac_weight(make_float2(m_lo, l_lo), M_lo), f_hi = ac_weight(make_float2(m_hi, l_hi), M_hi);
-  float* mo = (float*)ring_p + (long long)warp * 16 * HD;      // [16][HD]
+  float* mo = (float*)smem + warp * 16 * HD;           // [16][HD]
   if constexpr (!F32) {
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) {
@@ -523,7 +546,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int x = 0; x < G::NG; ++x) {
-      const float4 y = *(const float4*)((const float*)ring_p + ((long long)(x * R + tile) * 16 + rr) * HD + 4 * c);
+      const float4 y = *(const float4*)((const float*)smem + ((x * R + tile) * 16 + rr) * HD + 4 * c);
       a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
     }
     int b, t, h;

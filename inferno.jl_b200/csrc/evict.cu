@@ -28,8 +28,9 @@ namespace cg = cooperative_groups;
 
 constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_MOVE_THREADS = 256;
 constexpr int EV_BINS = 256;
-constexpr int EV_MAX_CLUSTER = 8;
+constexpr int EV_MAX_CLUSTER = 16;         // B200's largest, above the portable 8
 constexpr int EV_MAX_LEN = 1 << 21;         // the bitmaps of a CTA's part fit shared memory up to here
 constexpr int EV_SMEM = 200 * 1024;
 
@@ -47,6 +48,7 @@ struct EvictParams {
   int words;                          // 32-row words a CTA's part may have
   int cached;                         // keys held in shared memory
   int* lists;                         // [batch * nkv][2][max_moves]: holes, sources
+  int* counts;                        // [batch * nkv] rows to move; null: the clusters move K and V themselves
 };
 
 // larger is kept first; NaN below everything; -0 equal to 0
@@ -107,6 +109,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   float* so = p.scores_out + bh * p.stride;
   int* po = p.pos_out + bh * p.stride;
   if (len <= p.budget) {                      // the whole cluster leaves
+    if (p.counts && c == 0 && t == 0) p.counts[bh] = 0;
     for (int j = c * EV_THREADS + t; j < len; j += nc * EV_THREADS) {
       if (so != sc) so[j] = sc[j];
       if (po != ps) po[j] = ps[j];
@@ -317,6 +320,15 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   sync_all();                             // lists complete; also the last read of a peer's shared memory
 
   // ---- move ---------------------------------------------------------------------------
+  for (int i = c * EV_THREADS + t; i < moves; i += nc * EV_THREADS) {
+    const int from = src_list[i], to = hole_list[i];
+    so[to] = sc[from];
+    po[to] = ps[from];
+  }
+  if (p.counts) {
+    if (c == 0 && t == 0) p.counts[bh] = moves;
+    return;
+  }
   const int vecs = p.head_bytes / 16;         // 16-byte pieces of a K row; as many of the V row
   uint8_t* kb = p.kc + b * p.seq_bytes + (long long)h * p.head_bytes;
   uint8_t* vb = p.vc + b * p.seq_bytes + (long long)h * p.head_bytes;
@@ -343,17 +355,38 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
     for (int u = 0; u < U; ++u)
       if (to[u] >= 0) *(uint4*)((piece[u] < vecs ? kb + piece[u] * 16 : vb + (piece[u] - vecs) * 16) + to[u] * p.row_bytes) = x[u];
   }
-  for (int i = c * EV_THREADS + t; i < moves; i += nc * EV_THREADS) {
-    const int from = src_list[i], to = hole_list[i];
-    so[to] = sc[from];
-    po[to] = ps[from];
-  }
 }
 
-// lens_out in place: only once every cluster has read lens
-__global__ void evict_lens_kernel(int* lens, int batch, int max_len, int budget) {
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  if (b < batch) lens[b] = min(max(0, min(lens[b], max_len)), budget);
+// After evict_kernel: lens_out in place, once every cluster has read lens, and K and
+// V where there are too few (sequence, KV head) clusters to fill the GPU.
+__global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(const __grid_constant__ EvictParams p, int* lens, int rows_per_block) {
+  const int bh = blockIdx.y, b = bh / p.nkv, h = bh - b * p.nkv;
+  pdl_wait();
+  if (lens && blockIdx.x == 0 && h == 0 && threadIdx.x == 0) lens[b] = min(max(0, min(lens[b], p.max_len)), p.budget);
+  if (!p.counts) return;
+  const int r0 = blockIdx.x * rows_per_block, n = min(p.counts[bh] - r0, rows_per_block);
+  const int* holes = p.lists + (long long)bh * 2 * p.max_moves + r0;
+  const int* from = holes + p.max_moves;
+  const int vecs = p.head_bytes / 16;
+  uint8_t* kb = p.kc + b * p.seq_bytes + (long long)h * p.head_bytes;
+  uint8_t* vb = p.vc + b * p.seq_bytes + (long long)h * p.head_bytes;
+  constexpr int U = 8;
+  for (int i0 = threadIdx.x; i0 < n * 2 * vecs; i0 += U * EV_MOVE_THREADS) {
+    uint4 x[U];
+    uint8_t* dst[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * EV_MOVE_THREADS, row = i / (2 * vecs), piece = i - row * 2 * vecs;
+      dst[u] = nullptr;
+      if (row >= n) continue;
+      uint8_t* base = piece < vecs ? kb + piece * 16 : vb + (piece - vecs) * 16;
+      dst[u] = base + holes[row] * p.row_bytes;
+      x[u] = *(const uint4*)(base + from[row] * p.row_bytes);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (dst[u]) *(uint4*)dst[u] = x[u];
+  }
 }
 
 namespace {
@@ -385,7 +418,7 @@ int evict_check(const InfernoEvict* e) {
 int evict_max_moves(const InfernoEvict* e) { return std::max(0, std::min(e->budget, e->max_len - e->budget)); }
 
 int64_t evict_workspace(const InfernoEvict* e) {
-  return (int64_t)e->batch * e->n_kv_heads * 2 * evict_max_moves(e) * 4 + 256;
+  return (int64_t)e->batch * e->n_kv_heads * (2 * (int64_t)evict_max_moves(e) + 1) * 4 + 256;
 }
 
 }  // namespace
@@ -444,7 +477,7 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.max_moves = evict_max_moves(e);
   p.lists = (int*)workspace;
   if (e->lens_out == e->lens) p.lens_out = nullptr;
-  // CTAs per (sequence, KV head), up to 8 and while all run at once, two per SM: one
+  // CTAs per (sequence, KV head), up to 16 and while all run at once, two per SM: one
   // per 1024 rows to rank (4160 rows in 32 heads: 17.7 us with four, 20.6 with one,
   // which waits for itself instead of the others) or per 256 KB to move
   const int n = e->batch * e->n_kv_heads;
@@ -462,10 +495,16 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.cached = smem_of(nc, true) <= EV_SMEM;
   p.words = ((e->max_len + 31) / 32 + nc - 1) / nc;
   const size_t smem = smem_of(nc, p.cached);
+  // fewer than one CTA per SM and more than 1 MB to move: a second kernel over the
+  // whole GPU moves K and V (4 heads of 62898 fp32 rows of 128 to 14946: 105 us
+  // with the 32 CTAs alone)
+  const bool spread = n * nc < num_sms(dev) && 4ll * p.max_moves * p.head_bytes * n > (1 << 20);
+  if (spread) p.counts = (int*)workspace + (long long)n * 2 * p.max_moves;
   cudaStream_t st = (cudaStream_t)stream;
   static DeviceOnce once;
   cudaError_t err = once.run([] {
-    return cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
+    const cudaError_t a = cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
+    return a == cudaSuccess ? cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) : a;
   });
   if (err == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
@@ -481,9 +520,18 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
     cfg.numAttrs = 1;
     err = cudaLaunchKernelEx(&cfg, evict_kernel, p);
   }
-  if (err == cudaSuccess && !p.lens_out) {
-    evict_lens_kernel<<<(e->batch + 127) / 128, 128, 0, st>>>(e->lens_out, e->batch, e->max_len, e->budget);
-    err = cudaGetLastError();
+  if (err == cudaSuccess && (spread || !p.lens_out)) {
+    const int rows = std::max(1, (32 << 10) / p.head_bytes);         // 64 KB of K and V per block
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(spread ? (p.max_moves + rows - 1) / rows : 1), (unsigned)n);
+    cfg.blockDim = dim3(EV_MOVE_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    err = cudaLaunchKernelEx(&cfg, evict_move_kernel, p, p.lens_out ? nullptr : e->lens_out, rows);
   }
   return err == cudaSuccess ? 0 : set_error(INFERNO_ECUDA, "cache_evict launch: %s", cudaGetErrorString(err));
 }

@@ -212,6 +212,8 @@ ATTN = [
     ("f32", 3, 1, 16, 4, 256, 2048, 300, [300, 17, 129]),
     ("f32", 9, 2, 8, 2, 64, 333, 20, [2, 1, 0, 20, 5, 19, 16, 17, 18]),   # 72 prefix rows per KV head
     ("f32", 2, 3, 15, 3, 128, 65, 1000, [1000, 2]),                  # group 5; a token that sees no own row
+    ("f32", 5, 8, 5, 1, 128, 100, 90, [90, 40, 8, 3, 0]),            # 40 own rows: a row tile of the CTA is empty
+    ("f32", 7, 8, 4, 1, 256, 300, 40, [40] * 7),                     # 224 prefix rows
     ("bf16", 1, 1, 1, 1, 64, 1, 0, []),
     ("bf16", 5, 1, 16, 2, 128, 1000, 333, [333, 0, 128, 129, 1]),
     ("bf16", 33, 1, 8, 2, 256, 513, 33, list(range(33))),            # 132 prefix rows per KV head
@@ -394,6 +396,7 @@ EVICT = [
     ("bf16", 1, 2, 8, 3000, [3000], 2999, 0, 0),
     ("f32", 1, 1, 4, 5000, [5000], 1, 0, 1),
     ("f16", 4, 1, 80, 300, [0, -5, 400, 300], 150, 2, 10),           # lens are clamped
+    ("f32", 2, 1, 128, 6000, [6000, 2500], 3000, 4, 700),            # more to move than the clusters take
 ]
 
 
@@ -425,10 +428,11 @@ def test_evict_more_kept_always_than_budget():
     _check_evict(tid, k, v, scores, pos, [1200], [1200], budget=300, n_sink=1, n_recent=0)
 
 
-@pytest.mark.parametrize("rows,budget", [(40000, 9000), (400000, 100000)])
-def test_evict_long(rows, budget):
-    """Parts of a cluster that hold their keys in shared memory, and ones too long for it."""
-    tid, k, v, scores, pos = _evict_case("bf16", 1, 1, 8, rows, seed=7)
+@pytest.mark.parametrize("rows,budget,d", [(40000, 9000, 8), (30000, 12000, 256), (800000, 100000, 8)])
+def test_evict_long(rows, budget, d):
+    """Parts of a cluster that hold their keys in shared memory, rows that a second
+    kernel moves, and parts too long for shared memory."""
+    tid, k, v, scores, pos = _evict_case("bf16", 1, 1, d, rows, seed=7)
     _check_evict(tid, k, v, scores, pos, [rows - 3], [rows], budget=budget, n_sink=4, n_recent=budget // 3)
 
 
