@@ -33,10 +33,8 @@ namespace inf {
 namespace {
 
 constexpr int AC_KT = 16;                       // keys per tile
-constexpr int AC_SMEM = 227 * 1024, AC_SMEM_HALF = 113 * 1024;
+constexpr int AC_SMEM = 227 * 1024, AC_SMEM_HALF = 112 * 1024;
 constexpr int AC_FIN_THREADS = 256;
-constexpr int AC_FIN_PER = 4;                   // own rows per thread of a finishing CTA
-constexpr int AC_FIN_SLOTS = AC_FIN_THREADS * AC_FIN_PER;
 
 template <typename T>
 struct AcType;
@@ -133,10 +131,11 @@ __device__ __forceinline__ uint32_t tile_addr(uint32_t base, int r, int c) {
 // what a CTA works on
 struct AcWork {
   const uint8_t *k, *v;      // first key row of the KV head
+  long long entry;           // own part: entry of its first row
   int j0, j1;                // keys
   int row0, nrows;           // rows of this CTA among its part's; their number
   int b;                     // own part: the sequence (prefix: -1)
-  int kvh, split;            // split index among n_splits
+  int kvh, split;            // prefix: the split
   int len;                   // own part: lens[b]
 };
 
@@ -158,48 +157,126 @@ __device__ __forceinline__ float ac_weight(float2 ml, float M) {
   return ml.x == -INFINITY && ml.y == 0.f ? 0.f : exp2f(ml.x - M);
 }
 
-// blocks of a launch: the prefix part's, then the own part's; row tiles of each
+// CTAs of a launch: the prefix part's (row tiles of p_tiles), then the own part's
 struct AcGrid {
-  int p_blocks, p_tiles, o_tiles;
+  int p_blocks, p_tiles;
 };
 
-// the work of this CTA: rows_per_cta rows of a KV head against one split
+__device__ __forceinline__ int ac_len(const AcParams& p, int b) { return max(0, min(p.lens[b], p.max_len)); }
+__device__ __forceinline__ int ac_blocks(int len) { return (len + AC_BLOCK - 1) / AC_BLOCK; }
+
+// where an own-part CTA stands in the line of blocks (fewer than 2^30)
+struct AcCursor {
+  int pos, end;              // next block, end of the share
+  int before, b;             // blocks of the sequences before b
+  int group, u;              // the CTA's group and its KV head and row tile
+};
+
+// the segment at the cursor (sequence cur.b with `len` keys, up to the end of the
+// share), and the cursor past it
 template <typename T, int HD>
-__device__ __forceinline__ AcWork ac_work(const AcParams& p, AcGrid gr, int rows_per_cta) {
-  AcWork w;
+__device__ __forceinline__ void ac_take(const AcParams& p, AcCursor& cur, AcWork& w, int len) {
   constexpr int ROW = HD * (int)sizeof(T);
-  const bool prefix_part = (int)blockIdx.x < gr.p_blocks;
-  int x = prefix_part ? blockIdx.x : blockIdx.x - gr.p_blocks;
-  const int row_tiles = prefix_part ? gr.p_tiles : gr.o_tiles;
-  const int splits = prefix_part ? p.p_splits : p.o_splits;
-  w.split = x % splits;
-  x /= splits;
-  w.row0 = (x % row_tiles) * rows_per_cta;
-  x /= row_tiles;
-  w.kvh = x % p.nkv;
-  x /= p.nkv;
-  const int rows = p.n_tok * p.group;
-  if (prefix_part) {
-    w.b = -1;
-    w.nrows = p.batch * rows;
-    w.len = p.prefix_len;
-    w.j0 = w.split * p.p_split_len;
-    w.j1 = min(w.len, w.j0 + p.p_split_len);
-    w.k = (const uint8_t*)p.pk;
-    w.v = (const uint8_t*)p.pv;
-  } else {
-    w.b = x;
-    w.nrows = rows;
-    w.len = max(0, min(p.lens[x], p.max_len));
-    w.j0 = w.split * p.o_split_len;
-    w.j1 = min(w.len, w.j0 + p.o_split_len);
-    w.k = (const uint8_t*)p.kc + (long long)x * p.seq_stride * (int)sizeof(T);
-    w.v = (const uint8_t*)p.vc + (long long)x * p.seq_stride * (int)sizeof(T);
-    w.split += p.p_splits;
+  const int off = cur.pos - cur.before, n = min(ac_blocks(len) - off, cur.end - cur.pos);
+  cur.pos += n;
+  w.b = cur.b;
+  w.kvh = cur.u / p.o_tiles;
+  w.row0 = (cur.u - w.kvh * p.o_tiles) * p.o_rows;
+  w.nrows = p.n_tok * p.group;
+  w.len = len;
+  w.j0 = off * AC_BLOCK;
+  w.j1 = min(len, w.j0 + n * AC_BLOCK);
+  w.split = 0;
+  w.entry = p.own_base + ((long long)(cur.group + cur.b) * (p.nkv * p.o_tiles) + cur.u) * p.o_rows;
+  const long long base = (long long)cur.b * p.seq_stride * (int)sizeof(T) + (long long)w.kvh * ROW;
+  w.k = (const uint8_t*)p.kc + base;
+  w.v = (const uint8_t*)p.vc + base;
+}
+// the next segment; j0 = j1 when the share is done.  One thread.
+template <typename T, int HD>
+__device__ void ac_next(const AcParams& p, AcCursor& cur, AcWork& w) {
+  w.j0 = w.j1 = 0;
+  if (cur.pos >= cur.end) return;
+  int len = ac_len(p, cur.b);
+  while (cur.pos >= cur.before + ac_blocks(len)) {
+    cur.before += ac_blocks(len);
+    len = ac_len(p, ++cur.b);
   }
-  w.k += (long long)w.kvh * ROW;
-  w.v += (long long)w.kvh * ROW;
-  return w;
+  ac_take<T, HD>(p, cur, w, len);
+}
+
+// this CTA's first segment.  One warp; lane 0 leaves cursor and work.
+template <typename T, int HD>
+__device__ void ac_first(const AcParams& p, AcGrid gr, int rows_per_cta, AcCursor& cur, AcWork& w) {
+  const int lane = threadIdx.x & 31;
+  if ((int)blockIdx.x < gr.p_blocks) {
+    if (lane == 0) {
+      int x = blockIdx.x;
+      w.split = x % p.p_splits;
+      x /= p.p_splits;
+      w.row0 = (x % gr.p_tiles) * rows_per_cta;
+      w.kvh = x / gr.p_tiles;
+      w.b = -1;
+      w.nrows = p.batch * p.n_tok * p.group;
+      w.len = p.prefix_len;
+      w.j0 = w.split * p.p_split_len;
+      w.j1 = min(w.len, w.j0 + p.p_split_len);
+      w.entry = 0;
+      w.k = (const uint8_t*)p.pk + (long long)w.kvh * HD * (int)sizeof(T);
+      w.v = (const uint8_t*)p.pv + (long long)w.kvh * HD * (int)sizeof(T);
+      cur.pos = cur.end = 0;
+    }
+    return;
+  }
+  const int c = blockIdx.x - gr.p_blocks, units = p.nkv * p.o_tiles, group = c / units;
+  // lane l sums the blocks of `per` consecutive sequences
+  const int per = (p.batch + 31) / 32, b_lo = min(p.batch, lane * per), b_hi = min(p.batch, b_lo + per);
+  int mine = 0, len = 0;
+#pragma unroll 4
+  for (int b = b_lo; b < b_hi; ++b) {
+    len = ac_len(p, b);
+    mine += ac_blocks(len);
+  }
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  const int all = __shfl_sync(0xffffffffu, incl, 31);
+  const int share = max(1u, p.by_groups.div((uint32_t)(all + p.o_groups - 1)));
+  const int pos = group * share, end = min(all, pos + share);
+  if (c == 0) {
+    if (lane == 0) p.head[0] = share;
+    int before = incl - mine;
+    for (int b = b_lo; b < b_hi; ++b) {
+      p.head[1 + b] = before;
+      before += ac_blocks(ac_len(p, b));
+    }
+  }
+  if (pos >= end) {
+    if (lane == 0) w.j0 = w.j1 = 0;
+    return;
+  }
+  // the lane whose sequences hold pos
+  if (incl - mine <= pos && pos < incl) {
+    cur.group = group;
+    cur.u = c - group * units;
+    cur.pos = pos;
+    cur.end = end;
+    cur.before = incl - mine;
+    cur.b = b_lo;
+    if (per == 1) ac_take<T, HD>(p, cur, w, len);
+    else ac_next<T, HD>(p, cur, w);
+  }
+}
+
+// entry of row r (of the CTA's rows_per_cta) of a piece of work
+__device__ __forceinline__ long long ac_entry(const AcParams& p, const AcWork& w, int r) {
+  if (w.b >= 0) return w.entry + r;
+  int b, t, h;
+  ac_row(p, w, w.row0 + r, b, t, h);
+  return ((long long)(b * p.n_tok + t) * p.nh + h) * p.p_splits + w.split;
 }
 
 template <typename T, int HD, int R>
@@ -207,17 +284,19 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
   using G = AcGeo<T, HD, R>;
   constexpr bool F32 = AcType<T>::F32;
   constexpr int ROW = G::ROW, ITEM = G::ITEM, SLOTS = G::SLOTS, GT = R * 32;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int grp = warp / R, rt = warp - grp * R;       // key group, row tile of the warp
   const int gtid = tid - grp * GT;                     // thread within the group
 
+  __shared__ AcCursor s_cur;
+  __shared__ AcWork s_work;
   pdl_trigger();
-  const AcWork w = ac_work<T, HD>(p, gr, 16 * R);
-  if (w.j0 >= w.j1) {                // nothing of this sequence in this split
-    pdl_wait();
-    return;
-  }
+  if (warp == 0) ac_first<T, HD>(p, gr, 16 * R, s_cur, s_work);
+  for (;;) {
+  __syncthreads();
+  const AcWork w = s_work;
+  if (w.j0 >= w.j1) break;
   const long long key_stride = (long long)p.nkv * ROW;
 
   const uint32_t s_q = smem_u32(smem);                            // fp32 only: [16 R][HD]
@@ -549,9 +628,7 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
       const float4 y = *(const float4*)((const float*)smem + ((x * R + tile) * 16 + rr) * HD + 4 * c);
       a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
     }
-    int b, t, h;
-    ac_row(p, w, w.row0 + r, b, t, h);
-    const long long at = ((long long)(b * p.n_tok + t) * p.nh + h) * p.n_splits + w.split;
+    const long long at = ac_entry(p, w, r);
     *(float4*)(p.part_o + at * HD + 4 * c) = a;
     if (c == 0) {
       float M = -INFINITY, L = 0.f;
@@ -564,6 +641,9 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
       }
       p.part_ml[at] = make_float2(M, L);
     }
+  }
+  __syncthreads();                     // the merge buffer is the next segment's ring
+  if (tid == 0) ac_next<T, HD>(p, s_cur, s_work);
   }
   // launched beside the prefix part: not complete before it, so that the
   // finishing kernel, which waits for this one, finds both
@@ -600,11 +680,13 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
   __shared__ float s_q[RN][HD];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
-  const AcWork w = ac_work<float, HD>(p, gr, RN);
-  if (w.j0 >= w.j1) {
-    pdl_wait();
-    return;
-  }
+  __shared__ AcCursor s_cur;
+  __shared__ AcWork s_work;
+  if (warp == 0) ac_first<float, HD>(p, gr, RN, s_cur, s_work);
+  for (;;) {
+  __syncthreads();
+  const AcWork w = s_work;
+  if (w.j0 >= w.j1) break;
   const long long key_stride = (long long)p.nkv * HD;
   // dims of float2 i of this lane: pairs (0, 1) and (2, 3) are one 16-byte access
   auto dim = [&](int i) { return 128 * (i >> 1) + 4 * lane + 2 * (i & 1); };
@@ -736,9 +818,7 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
       const float4 y = *(const float4*)&merge[x][r][4 * c];
       a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
     }
-    int b, t, h;
-    ac_row(p, w, w.row0 + r, b, t, h);
-    const long long at = ((long long)(b * p.n_tok + t) * p.nh + h) * p.n_splits + w.split;
+    const long long at = ac_entry(p, w, r);
     *(float4*)(p.part_o + at * HD + 4 * c) = a;
     if (c == 0) {
       float M = -INFINITY, L = 0.f;
@@ -749,44 +829,68 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
       p.part_ml[at] = make_float2(M, L);
     }
   }
+  __syncthreads();
+  if (tid == 0) ac_next<float, HD>(p, s_cur, s_work);
+  }
   pdl_wait();                          // see ac_part_kernel
 }
 
-// splits of a row that hold something: all of the prefix, own ones up to lens
-__device__ __forceinline__ int ac_live_splits(const AcParams& p, int b) {
-  int n = p.p_splits;
-  if (p.o_splits) {
-    const int len = max(0, min(p.lens[b], p.max_len));
-    n += (len + p.o_split_len - 1) / p.o_split_len;
+// the partials of a row: p_splits of the prefix, then those of the own part's CTAs
+struct AcParts {
+  long long prefix, own, step;     // first entries; between the own part's
+  int n, p_splits;
+  __device__ __forceinline__ long long at(int s) const { return s < p_splits ? prefix + s : own + (s - p_splits) * step; }
+};
+// row r of sequence b and KV head kvh (t * group + g), `row` over all
+__device__ __forceinline__ AcParts ac_parts(const AcParams& p, int b, int kvh, int r, long long row) {
+  AcParts x;
+  x.p_splits = x.n = p.p_splits;
+  x.prefix = row * p.p_splits;
+  x.own = x.step = 0;
+  if (p.o_groups) {
+    const int nb = ac_blocks(ac_len(p, b)), tile = r / p.o_rows, units = p.nkv * p.o_tiles;
+    if (nb) {
+      const int share = p.head[0], pos = p.head[1 + b];
+      const int c0 = pos / share, c1 = (pos + nb - 1) / share;
+      x.own = p.own_base + ((long long)(c0 + b) * units + kvh * p.o_tiles + tile) * p.o_rows + (r - tile * p.o_rows);
+      x.step = (long long)units * p.o_rows;
+      x.n += c1 - c0 + 1;
+    }
   }
-  return n;
+  return x;
 }
-// (largest logit, 1 / sum) over a row's splits; called by a whole warp
-__device__ __forceinline__ float2 ac_row_stats(const AcParams& p, long long row, int n) {
-  const float2* ml = p.part_ml + row * p.n_splits;
-  float M = -INFINITY;
-  for (int s = threadIdx.x & 31; s < n; s += 32) M = fmaxf(M, ml[s].x);
-  M = warp_max(M);
-  float L = 0.f;
-  for (int s = threadIdx.x & 31; s < n; s += 32) {
-    const float2 x = ml[s];
-    L += x.y * ac_weight(x, M);
+// (largest logit, 1 / sum) over a row's partials; called by a whole warp
+__device__ __forceinline__ float2 ac_row_stats(const AcParams& p, const AcParts& parts) {
+  const int lane = threadIdx.x & 31;
+  float M = -INFINITY, L = 0.f;
+  for (int s0 = 0; s0 < parts.n; s0 += 128) {        // 128 partials' loads in flight
+    float2 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i * 32 + lane;
+      x[i] = s < parts.n ? p.part_ml[parts.at(s)] : make_float2(-INFINITY, 0.f);
+    }
+    const float m = warp_max(fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x))), n = fmaxf(M, m);
+    float l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l += x[i].y * ac_weight(x[i], n);
+    L = L * ac_weight(make_float2(M, L), n) + warp_sum(l);
+    M = n;
   }
-  L = warp_sum(L);
   return make_float2(M, L > 0.f ? 1.f / L : (L == L ? 0.f : L));
 }
 
 // blocks [0, row_blocks): W warps per row join its splits (every W-th one each,
-// then one another's sums in warp order), all loads of a warp in flight; blocks
-// behind: `scores` of one (sequence, KV head), AC_FIN_SLOTS own rows each
-template <typename T, int HD, int W>
-__global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_constant__ AcParams p, int row_blocks, int slot_blocks) {
+// then one another's sums in warp order), the loads of several in flight; blocks
+// behind: `scores` of one (sequence, KV head), SLOTS own rows per thread
+template <typename T, int HD, int W, int SLOTS>
+__global__ void __launch_bounds__(AC_FIN_THREADS, 4) ac_finish_kernel(const __grid_constant__ AcParams p, int row_blocks, int slot_blocks) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int WARPS = AC_FIN_THREADS / 32;
   pdl_wait();
   if (blockIdx.x < row_blocks) {
     constexpr int PER = HD / 32;                     // dims of a lane
-    constexpr int U = 16 / PER < 4 ? 4 : 16 / PER;   // splits in flight
+    constexpr int U = 32 / PER;                      // partials in flight
     __shared__ float part[W > 1 ? WARPS : 1][HD];
     const long long row = (long long)blockIdx.x * (WARPS / W) + warp / W;
     const long long tok = row / p.nh;
@@ -798,11 +902,12 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
     for (int i = 0; i < PER; ++i) a[i] = 0.f;
     float inv = 0.f;
     if (live) {
-      const int n = ac_live_splits(p, (int)(tok / p.n_tok));
-      const float2 st = ac_row_stats(p, row, n);
+      const int b = (int)(tok / p.n_tok), t = (int)(tok - (long long)b * p.n_tok), kvh = (int)p.by_group.div(h);
+      const AcParts parts = ac_parts(p, b, kvh, t * p.group + h - kvh * p.group, row);
+      const int n = parts.n;
+      const float2 st = ac_row_stats(p, parts);
       inv = st.y;
-      const float2* ml = p.part_ml + row * p.n_splits;
-      const float* o = p.part_o + row * p.n_splits * HD + lane * PER;
+      const float* o = p.part_o + lane * PER;
       for (int s0 = sub; s0 < n; s0 += U * W) {
         float f[U], x[U][PER];
 #pragma unroll
@@ -810,10 +915,11 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
           const int s = s0 + u * W;
           f[u] = 0.f;
           if (s < n) {
-            f[u] = ac_weight(ml[s], st.x);
+            const long long at = parts.at(s);
+            f[u] = ac_weight(p.part_ml[at], st.x);
 #pragma unroll
             for (int i = 0; i < PER; i += 2) {
-              const float2 y = *(const float2*)(o + (long long)s * HD + i);
+              const float2 y = *(const float2*)(o + at * HD + i);
               x[u][i] = y.x, x[u][i + 1] = y.y;
             }
           } else {
@@ -847,45 +953,71 @@ __global__ void __launch_bounds__(AC_FIN_THREADS) ac_finish_kernel(const __grid_
     return;
   }
   constexpr int CHUNK = 64;                          // rows whose statistics are held at once
-  constexpr int U = 4;                               // rows whose logits are in flight
+  constexpr int U = 16 / SLOTS;                      // rows whose logits are in flight
   __shared__ float2 st[CHUNK];
   __shared__ long long at[CHUNK];                    // the rows' logits
   const int x = blockIdx.x - row_blocks, bh = x / slot_blocks, b = bh / p.nkv, kvh = bh - b * p.nkv;
-  const int j0 = (x - bh * slot_blocks) * AC_FIN_SLOTS + threadIdx.x;
-  const int len = max(0, min(p.lens[b], p.max_len));
+  const int j0 = (x - bh * slot_blocks) * (AC_FIN_THREADS * SLOTS) + threadIdx.x;
+  const int len = ac_len(p, b);
   if (j0 - (int)threadIdx.x >= len) return;
-  const int n = ac_live_splits(p, b), rows = p.n_tok * p.group;
-  float sum[AC_FIN_PER];
+  const int rows = p.n_tok * p.group;
+  float sum[SLOTS];
 #pragma unroll
-  for (int i = 0; i < AC_FIN_PER; ++i) sum[i] = 0.f;
+  for (int i = 0; i < SLOTS; ++i) sum[i] = 0.f;
   for (int r0 = 0; r0 < rows; r0 += CHUNK) {
     const int nr = min(CHUNK, rows - r0);
+    // 32, 16, 8 or 4 lanes per row, so that all rows go at once
+    const int tpr = nr <= WARPS ? 32 : nr <= 2 * WARPS ? 16 : nr <= 4 * WARPS ? 8 : 4;
     __syncthreads();
-    for (int r = warp; r < nr; r += AC_FIN_THREADS / 32) {
-      const int t = (r0 + r) / p.group, h = kvh * p.group + (r0 + r) - t * p.group;
+    {
+      const int r = threadIdx.x / tpr, sub = threadIdx.x & (tpr - 1), rr = r0 + min(r, nr - 1);
+      const int t = (int)p.by_group.div(rr), h = kvh * p.group + rr - t * p.group;
       const long long row = (long long)(b * p.n_tok + t) * p.nh + h;
-      const float2 s = ac_row_stats(p, row, n);
-      if (lane == 0) st[r] = s, at[r] = row * p.logit_stride;
+      const AcParts parts = ac_parts(p, b, kvh, rr, row);
+      float M = -INFINITY, L = 0.f;
+      for (int s0 = 0; s0 < parts.n; s0 += 4 * tpr) {
+        float2 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int s = s0 + i * tpr + sub;
+          y[i] = s < parts.n ? p.part_ml[parts.at(s)] : make_float2(-INFINITY, 0.f);
+        }
+        const float m = fmaxf(M, fmaxf(fmaxf(y[0].x, y[1].x), fmaxf(y[2].x, y[3].x)));
+        float l = L * ac_weight(make_float2(M, L), m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l += y[i].y * ac_weight(y[i], m);
+        M = m, L = l;
+      }
+      for (int o = 1; o < tpr; o <<= 1) {
+        const float2 y = make_float2(__shfl_xor_sync(0xffffffffu, M, o), __shfl_xor_sync(0xffffffffu, L, o));
+        const float m = fmaxf(M, y.x);
+        L = L * ac_weight(make_float2(M, L), m) + y.y * ac_weight(y, m);
+        M = m;
+      }
+      if (sub == 0 && r < nr) {
+        st[r] = make_float2(M, L > 0.f ? 1.f / L : (L == L ? 0.f : L));
+        at[r] = row * p.logit_stride;
+      }
     }
     __syncthreads();
     for (int r = 0; r < nr; r += U) {
-      float lg[U][AC_FIN_PER];
+      float lg[U][SLOTS];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < AC_FIN_PER; ++i) {
+        for (int i = 0; i < SLOTS; ++i) {
           const int j = j0 + i * AC_FIN_THREADS;
           lg[u][i] = r + u < nr && j < len ? p.logits[at[r + u] + j] : -INFINITY;
         }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < AC_FIN_PER; ++i)
+        for (int i = 0; i < SLOTS; ++i)
           if (lg[u][i] != -INFINITY) sum[i] += exp2f(lg[u][i] - st[r + u].x) * st[r + u].y;
     }
   }
 #pragma unroll
-  for (int i = 0; i < AC_FIN_PER; ++i) {
+  for (int i = 0; i < SLOTS; ++i) {
     const int j = j0 + i * AC_FIN_THREADS;
     if (j < len) p.scores[(long long)bh * p.score_stride + j] += sum[i];
   }
@@ -897,7 +1029,7 @@ struct AcPlan {
   int p_r, o_r;                   // rows per CTA of the two parts: 16, 32, 64 (ac_part_kernel), 4, 8 (ac_vec_kernel)
   int p_tiles;                    // row tiles of the prefix part
   long long rows;                 // query rows over all heads
-  size_t off_ml, off_logits, bytes;
+  size_t off_ml, off_head, off_logits, bytes;
 };
 
 // Rows per CTA for a part with `rows` query rows per KV head and `len` keys.  fp32
@@ -912,17 +1044,11 @@ int ac_row_class(int type, int hd, long long rows, int len) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
-// Splits of `len` keys when `units` (KV heads x row tiles x sequences) share the
-// GPU: about four rounds of two CTAs per SM, which evens out ragged lengths, as
-// long as a split keeps 256 keys (below that starting and merging a CTA costs more
-// than it streams); with fewer keys, one round, down to 64 keys, one tile of 16
-// for each of the four key groups.
+// Splits of the prefix when `units` (KV heads x row tiles) share the GPU: about four
+// rounds of two CTAs per SM as long as a split keeps 256 keys (below that starting
+// and merging a CTA costs more than it streams); with fewer keys, one round, down
+// to 64 keys, one tile of 16 for each of four key groups.
 void ac_split(long long units, long long len, int* splits, int* split_len) {
-  if (len <= 0) {
-    *splits = 0;
-    *split_len = 64;
-    return;
-  }
   auto keys = [&](long long ctas) {
     const long long want = std::max(1ll, std::min(256ll, ctas / units));
     return ((len + want - 1) / want + 63) / 64 * 64;
@@ -930,6 +1056,17 @@ void ac_split(long long units, long long len, int* splits, int* split_len) {
   const long long sl = std::max(keys(4 * 296), std::min(256ll, keys(296)));
   *split_len = (int)sl;
   *splits = (int)((len + sl - 1) / sl);
+}
+
+template <typename T, int HD>
+int ac_ctas_per_sm(int r) {
+  if (r <= 8) return HD == 256 ? 2 : 3;                    // ac_vec_kernel
+  return r == 16 ? AcGeo<T, HD, 1>::CTAS : r == 32 ? AcGeo<T, HD, 2>::CTAS : AcGeo<T, HD, 4>::CTAS;
+}
+int ac_ctas_per_sm(int type, int hd, int r) {
+  if (type == INFERNO_F32)
+    return hd == 64 ? ac_ctas_per_sm<float, 64>(r) : hd == 128 ? ac_ctas_per_sm<float, 128>(r) : ac_ctas_per_sm<float, 256>(r);
+  return hd == 64 ? ac_ctas_per_sm<__half, 64>(r) : hd == 128 ? ac_ctas_per_sm<__half, 128>(r) : ac_ctas_per_sm<__half, 256>(r);
 }
 
 // The prefix part on tcgen05: 16-bit types with more rows than two tiles of 16
@@ -952,6 +1089,8 @@ int ac_check(const InfernoAttention* a) {
   if (a->prefix_len > (1 << 30) || a->max_len > (1 << 30) || a->n_heads > 65536 ||
       (double)a->batch * a->n_tokens * a->n_heads > (double)(1 << 24))
     return set_error(INFERNO_EINVAL, "attention_cached: more than 2^24 query rows or 2^30 keys");
+  if ((double)a->batch * (a->max_len / AC_BLOCK + 1) > (double)(1 << 30))
+    return set_error(INFERNO_EINVAL, "attention_cached: more than 2^30 blocks of %d keys", AC_BLOCK);
   if (!std::isfinite(a->scale)) return set_error(INFERNO_EINVAL, "attention_cached: scale is not finite");
   return 0;
 }
@@ -976,10 +1115,13 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   if (a->prefix_len && a->max_len && pl.p_r > pl.o_r && (pl.p_r <= 8 || pl.o_r >= 16) && !ac_prefix_tc(a->type, pre) &&
       (long long)a->max_len * a->batch <= a->prefix_len)
     pl.o_r = pl.p_r;
-  const int o_tiles = (int)((own + pl.o_r - 1) / pl.o_r);
+  p->o_rows = pl.o_r;
+  p->o_tiles = (int)((own + pl.o_r - 1) / pl.o_r);
   pl.p_tiles = (int)((pre + pl.p_r - 1) / pl.p_r);
+  p->p_splits = 0;
   pl.p_tc = ac_prefix_tc(a->type, pre);
-  if (pl.p_tc) {
+  if (!a->prefix_len) {
+  } else if (pl.p_tc) {
     // one round of CTAs: splits of at least two tiles
     pl.p_tiles = (int)((pre + ap_rows() - 1) / ap_rows());
     const long long units = (long long)pl.p_tiles * a->n_kv_heads;
@@ -990,12 +1132,20 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   } else {
     ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, &p->p_splits, &p->p_split_len);
   }
-  ac_split((long long)o_tiles * a->n_kv_heads * a->batch, a->max_len, &p->o_splits, &p->o_split_len);
-  p->n_splits = p->p_splits + p->o_splits;
+  // own part: as many groups of CTAs as fit the GPU at once (two rounds where a
+  // group is large, whose remainder would idle), a block of keys each at least
+  const long long units = (long long)a->n_kv_heads * p->o_tiles;
+  const long long blocks = (long long)a->batch * ((a->max_len + AC_BLOCK - 1) / AC_BLOCK);
+  const long long at_once = 148ll * ac_ctas_per_sm(a->type, a->head_dim, pl.o_r);
+  p->o_groups = (int)std::min(blocks, units <= at_once / 8 ? at_once / units : (2 * at_once + units - 1) / units);
+  p->by_groups = FastDiv((uint32_t)std::max(1, p->o_groups));
+  p->own_base = pl.rows * p->p_splits;
+  const long long entries = p->own_base + (p->o_groups ? (p->o_groups + a->batch) * units * pl.o_r : 0);
   p->logit_stride = a->scores ? ((long long)a->max_len + 15) / 16 * 16 : 0;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  pl.off_ml = up((size_t)pl.rows * p->n_splits * a->head_dim * 4);
-  pl.off_logits = pl.off_ml + up((size_t)pl.rows * p->n_splits * 8);
+  pl.off_ml = up((size_t)entries * a->head_dim * 4);
+  pl.off_head = pl.off_ml + up((size_t)entries * 8);
+  pl.off_logits = pl.off_head + up((size_t)(1 + a->batch) * 4);
   pl.bytes = pl.off_logits + up((size_t)pl.rows * p->logit_stride * 4) + 256;
   return pl;
 }
@@ -1032,11 +1182,10 @@ cudaError_t ac_launch_part(const AcParams& p, AcGrid gr, long long blocks, bool 
 // one kernel over the prefix part, the own part or both, r rows per CTA
 template <typename T, int HD>
 cudaError_t ac_part(const AcParams& p, const AcPlan& pl, int r, bool prefix, bool own, bool beside, cudaStream_t st) {
-  const long long pt = ((long long)p.batch * p.n_tok * p.group + r - 1) / r, ot = ((long long)p.n_tok * p.group + r - 1) / r;
-  const long long pb = prefix ? pt * p.nkv * p.p_splits : 0;
-  const long long blocks = pb + (own ? ot * p.nkv * p.o_splits * p.batch : 0);
+  const long long pb = prefix ? (long long)pl.p_tiles * p.nkv * p.p_splits : 0;
+  const long long blocks = pb + (own ? (long long)p.o_groups * p.nkv * p.o_tiles : 0);
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  const AcGrid gr{(int)pb, (int)pt, (int)ot};
+  const AcGrid gr{(int)pb, pl.p_tiles};
   if constexpr (AcType<T>::F32 && HD >= 128) {
     if (r == 4) return ac_launch(ac_vec_kernel<HD, 4>, blocks, AV_WARPS * 32, 0, st, beside, p, gr);
   }
@@ -1051,7 +1200,7 @@ template <typename T, int HD>
 cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   bool any = pl.p_tc && p.p_splits;    // a kernel of this call is in flight
-  const bool prefix = p.p_splits && !pl.p_tc, own = p.o_splits > 0;
+  const bool prefix = p.p_splits && !pl.p_tc, own = p.o_groups > 0;
   if (prefix && own && pl.p_r == pl.o_r) {
     e = ac_part<T, HD>(p, pl, pl.p_r, true, true, false, st);
     any = true;
@@ -1066,14 +1215,20 @@ cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
     }
   }
   if (e != cudaSuccess) return e;
-  // four warps per row when it has more splits than one warp has in flight
-  const bool wide = p.n_splits > 8;
-  const int per_block = AC_FIN_THREADS / 32 / (wide ? 4 : 1);
+  // warps per row by its partials, one warp having 4 to 16 in flight; the own part's
+  // are about as many as groups per sequence
+  const long long parts = p.p_splits + (p.o_groups ? 1 + p.o_groups / p.batch : 0);
+  const int warps = parts <= 8 ? 1 : parts <= 24 ? 4 : 8;
+  const int per_block = AC_FIN_THREADS / 32 / warps;
   const long long row_blocks = (pl.rows + per_block - 1) / per_block;
-  const long long slot_blocks = p.scores ? (p.max_len + AC_FIN_SLOTS - 1) / AC_FIN_SLOTS : 0;
-  const long long blocks = row_blocks + slot_blocks * p.batch * p.nkv;
-  return ac_launch(wide ? ac_finish_kernel<T, HD, 4> : ac_finish_kernel<T, HD, 1>, blocks, AC_FIN_THREADS, 0, st, any, p,
-                   (int)row_blocks, (int)std::max(1ll, slot_blocks));
+  // four cache rows per thread, or one where that leaves fewer than two CTAs per SM
+  const long long heads = (long long)p.batch * p.nkv;
+  const int slots = p.scores && heads * ((p.max_len + 4 * AC_FIN_THREADS - 1) / (4 * AC_FIN_THREADS)) >= 296 ? 4 : 1;
+  const long long slot_blocks = p.scores ? (p.max_len + slots * AC_FIN_THREADS - 1) / (slots * AC_FIN_THREADS) : 0;
+  const long long blocks = row_blocks + slot_blocks * heads;
+  auto* kernel = slots == 4 ? (warps == 1 ? ac_finish_kernel<T, HD, 1, 4> : warps == 4 ? ac_finish_kernel<T, HD, 4, 4> : ac_finish_kernel<T, HD, 8, 4>)
+                            : (warps == 1 ? ac_finish_kernel<T, HD, 1, 1> : warps == 4 ? ac_finish_kernel<T, HD, 4, 1> : ac_finish_kernel<T, HD, 8, 1>);
+  return ac_launch(kernel, blocks, AC_FIN_THREADS, 0, st, any, p, (int)row_blocks, (int)std::max(1ll, slot_blocks));
 }
 template <typename T>
 cudaError_t ac_run_hd(int hd, const AcParams& p, const AcPlan& pl, cudaStream_t st) {
@@ -1140,6 +1295,7 @@ extern "C" int inferno_attention_cached(const InfernoAttention* a, void* workspa
   p.scale_log2 = (a->scale == 0.0f ? 1.0f / sqrtf((float)a->head_dim) : a->scale) * AC_LOG2E;
   p.part_o = (float*)workspace;
   p.part_ml = (float2*)((char*)workspace + pl.off_ml);
+  p.head = (int*)((char*)workspace + pl.off_head);
   p.logits = (float*)((char*)workspace + pl.off_logits);
   cudaStream_t st = (cudaStream_t)stream;
   if (pl.p_tc && p.p_splits && (rc = launch_attn_prefix_tc(a->type, a->head_dim, p, pl.p_tiles, st))) return rc;

@@ -7,9 +7,19 @@
 
 namespace inf {
 
-// Query rows are numbered r = (b * n_tokens + t) * n_heads + h.  Every split of
-// the keys leaves, per row, its largest logit and the sum and weighted V sum of
-// exp2(logit - largest); logits are in units of log2.
+// Query rows are numbered r = (b * n_tokens + t) * n_heads + h.  A CTA leaves, for
+// each of its rows, one partial result over its keys: the largest logit and the sum
+// and weighted V sum of exp2(logit - largest); logits are in units of log2.
+//
+// The prefix is cut into p_splits equal splits; row r's partial of split s is entry
+// r * p_splits + s.  The own parts are cut evenly whatever lens are: keys are counted
+// in blocks of AC_BLOCK, the sequences' blocks stand in one line, and group c of
+// o_groups takes `share` blocks of it from c * share on, with one CTA for each unit:
+// a KV head and a row tile of o_rows rows.  (The CTAs of a group walk the same keys
+// side by side, so that the heads' parts of a cache row are read together.)  Along
+// the line either the group or the sequence steps, so group c's partials of sequence
+// b are slot c + b: units * o_rows entries from own_base on.  head holds share and
+// the blocks before each sequence.
 struct AcParams {
   const void* q;
   const void *pk, *pv;           // shared prefix [prefix_len][nkv][hd]
@@ -20,16 +30,19 @@ struct AcParams {
   long long q_stride, out_stride, seq_stride, score_stride;   // elements
   int batch, n_tok, nh, nkv, group, prefix_len, max_len;
   FastDiv by_seq, by_group;      // a sequence's rows of one KV head, n_tok * group; group
+  FastDiv by_groups;             // o_groups
   float scale_log2;              // scale * log2(e)
-  // splits: prefix splits come first, then own ones; split s of a part covers
-  // its keys [s * len, (s + 1) * len)
-  int p_splits, p_split_len, o_splits, o_split_len, n_splits;
-  float* part_o;                 // [row][n_splits][hd]
-  float2* part_ml;               // [row][n_splits] (largest logit, sum)
+  int p_splits, p_split_len;     // split s: keys [s * len, (s + 1) * len)
+  int o_rows, o_tiles, o_groups;
+  long long own_base;
+  float* part_o;                 // [entry][hd]
+  float2* part_ml;               // [entry] (largest logit, sum)
+  int* head;                     // [1 + batch]
   float* logits;                 // [row][logit_stride] own logits (only with scores)
   long long logit_stride;
 };
 
+constexpr int AC_BLOCK = 64;
 constexpr float AC_LOG2E = 1.4426950408889634f;
 
 // 16 bytes to shared memory, zeros where not valid (src is then not read)

@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         const int r = row0 + warp * 32 + i * 4 + (lane >> 3);
         int tok, h;
         ap_row(p, kvh, r, tok, h);
-        at[i] = r < nrows ? ((long long)tok * p.nh + h) * p.n_splits + split : -1;
+        at[i] = r < nrows ? ((long long)tok * p.nh + h) * p.p_splits + split : -1;
       }
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       if (r < nrows) {
         int tok, h;
         ap_row(p, kvh, r, tok, h);
-        p.part_ml[((long long)tok * p.nh + h) * p.n_splits + split] = make_float2(m, l);
+        p.part_ml[((long long)tok * p.nh + h) * p.p_splits + split] = make_float2(m, l);
       }
     }
   }
