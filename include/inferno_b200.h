@@ -244,8 +244,9 @@ int inferno_rope(const InfernoRope* r, void* stream);
  *   out = sum_j p_j v_j, p = softmax_j(scale q . k_j) over both parts
  * Query head h reads KV head h / (n_heads / n_kv_heads); no RoPE, norm or gate
  * is applied.  A token that sees no row gets zeros.  lens are clamped to
- * [0, max_len]; rows from lens[b] on are not read as values, whatever they
- * hold.  Non-finite values in rows that are seen give non-finite outputs.
+ * [0, max_len].  Rows that a token does not see do not reach its output,
+ * whatever they hold (rows from lens[b] on, and those of the tokens behind it);
+ * non-finite values in rows that it sees make its output non-finite.
  * scores (optional, fp32): scores[(b * n_kv_heads + h) * score_stride + j]
  * gains the weight that own row j got, summed over the tokens and query heads
  * of KV head h; entries from lens[b] on are left as they are.

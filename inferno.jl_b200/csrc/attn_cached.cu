@@ -21,6 +21,7 @@
 // rows to `scores` from the logits that the first kernel left.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include "internal.h"
 #include "common.cuh"
@@ -126,6 +127,26 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <int ROW>
 __device__ __forceinline__ uint32_t tile_addr(uint32_t base, int r, int c) {
   return base + r * ROW + ((c ^ (r & 7)) << 4);
+}
+
+// bit k: row k of a tile (AC_KT rows of V) holds an infinity or NaN.  A whole warp.
+template <typename T, int ROW>
+__device__ __forceinline__ uint32_t ac_bad_rows(uint32_t tile, int lane) {
+  constexpr int CH = ROW / 16;
+  uint32_t bad = 0;
+  for (int id = lane; id < AC_KT * CH; id += 32) {
+    const float4 f = lds_f4(tile + id * 16);        // swizzled within the row: any order does
+    const uint32_t x[4] = {__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)};
+    bool is = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, float>) is |= (x[i] & 0x7f800000u) == 0x7f800000u;
+      else if constexpr (std::is_same_v<T, __half>) is |= (x[i] & 0x7c00u) == 0x7c00u || (x[i] & 0x7c000000u) == 0x7c000000u;
+      else is |= (x[i] & 0x7f80u) == 0x7f80u || (x[i] & 0x7f800000u) == 0x7f800000u;
+    }
+    if (is) bad |= 1u << (id / CH);
+  }
+  return __reduce_or_sync(0xffffffffu, bad);
 }
 
 // what a CTA works on
@@ -528,15 +549,29 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
     landed();
     issue(2 * i + 1 + SLOTS - 1);
     const uint32_t vt = ring + ((2 * i + 1) % SLOTS) * ITEM;
+    // Rows of the call's own tokens, which the tokens before them do not see, may
+    // hold anything (padding): 0 times infinity would reach those.  Such rows of V
+    // count as zeros, and the rows of Q that do see them become NaN.
+    uint32_t bad = 0;
+    if (w.b >= 0 && key0 + AC_KT > w.len - p.n_tok + 1 && p.n_tok > 1) {
+      bad = ac_bad_rows<T, ROW>(vt, lane);
+      const uint32_t z_lo = lim_lo <= key0 ? 0u : (1u << min(16, lim_lo - key0)) - 1, z_hi = lim_hi <= key0 ? 0u : (1u << min(16, lim_hi - key0)) - 1;
+      if (bad & z_lo) l_lo = NAN;
+      if (bad & z_hi) l_hi = NAN;
+    }
     if constexpr (!F32) {
       // P rounded to the 16-bit type, as V is: half a step (2^-9, 2^-12) per
       // term, below the rounding of the output
       const uint32_t pa[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
                               pack2<T>(s[1][2], s[1][3])};
+      // keys 2 t4, 2 t4 + 1 and 8 more of this thread's V values
+      const uint32_t k0 = bad >> (2 * t4), k1 = bad >> (8 + 2 * t4);
+      const uint32_t z0 = (k0 & 1 ? 0u : 0xffffu) | (k0 & 2 ? 0u : 0xffff0000u), z1 = (k1 & 1 ? 0u : 0xffffu) | (k1 & 2 ? 0u : 0xffff0000u);
 #pragma unroll
       for (int n = 0; n < HD / 16; ++n) {
         uint32_t vb[4];
         ldsm_x4_t(tile_addr<ROW>(vt, ((lane >> 3) & 1) * 8 + (lane & 7), 2 * n + (lane >> 4)), vb);
+        if (bad) vb[0] &= z0, vb[1] &= z1, vb[2] &= z0, vb[3] &= z1;
         mma16<T>(o[2 * n], pa, vb[0], vb[1]);
         mma16<T>(o[2 * n + 1], pa, vb[2], vb[3]);
       }
@@ -559,8 +594,12 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           // dims 32 cg + 4 g + x are column g of n tile 4 cg + x
-          const float4 v0 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4, 8 * cg + g));
-          const float4 v1 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4 + 1, 8 * cg + g));
+          float4 v0 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4, 8 * cg + g));
+          float4 v1 = lds_f4(tile_addr<ROW>(vt, 8 * n + 2 * t4 + 1, 8 * cg + g));
+          if (bad) {
+            if (bad >> (8 * n + 2 * t4) & 1) v0 = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (bad >> (8 * n + 2 * t4 + 1) & 1) v1 = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
           const float a[4] = {v0.x, v0.y, v0.z, v0.w}, b[4] = {v1.x, v1.y, v1.z, v1.w};
           uint32_t h[4][2], lo[4][2];
 #pragma unroll
@@ -783,6 +822,20 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
     }
     const float pr = exp2f(x - (m == -INFINITY ? 0.f : m));
     l += pr;
+    if (w.b >= 0 && p.n_tok > 1 && key0 + KT > w.len - p.n_tok + 1) {
+      // rows of the call's own tokens: as in ac_part_kernel
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        bool is = false;
+#pragma unroll
+        for (int i = 0; i < D2; ++i) is |= !(fabsf(vx[k][i].x) < INFINITY) || !(fabsf(vx[k][i].y) < INFINITY);
+        if (__any_sync(0xffffffffu, is)) {
+#pragma unroll
+          for (int i = 0; i < D2; ++i) vx[k][i] = make_float2(0.f, 0.f);
+          if (my_key == k && key < lim) l = NAN;
+        }
+      }
+    }
     // ---- O += P V ----
 #pragma unroll
     for (int k = 0; k < KT; ++k)

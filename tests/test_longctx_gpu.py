@@ -298,6 +298,21 @@ def test_attention_nan_rows_stay_apart():
     assert nan[2, 0, 3].all() and not nan[2, 0, :3].any() and not nan[0].any()
 
 
+@pytest.mark.parametrize("dtype,H,d,T", [("f32", 1, 256, 4), ("f32", 2, 128, 2), ("f32", 3, 64, 5), ("f32", 6, 256, 5),
+                                         ("bf16", 2, 128, 3), ("f16", 8, 64, 4), ("bf16", 4, 256, 20)])
+def test_attention_padded_tokens(dtype, H, d, T):
+    """The rows of the last tokens hold garbage (padding): the tokens before them
+    get what they get from clean rows, bit for bit, those that see them NaN."""
+    tid, c, L = _attn_case(dtype, 3, T, 2 * H, 2, d, 40, 90, [90, 33, T], seed=4, weights=True)
+    clean = {n: x.clone() if n in ("out", "scores") else x for n, x in c.items()}
+    R.attention(R.attention_args(tid, max_len=L, **clean))
+    for b, n in enumerate([90, 33, T]):
+        c["k"][b, n - 1], c["v"][b, n - 1] = NAN, float("inf")
+    R.attention(R.attention_args(tid, max_len=L, **c))
+    assert torch.equal(c["out"][:, :-1], clean["out"][:, :-1])
+    assert c["out"][:, -1].isnan().all()
+
+
 def test_attention_repeats_bit_for_bit():
     for dtype, P in (("f32", 700), ("bf16", 3001)):
         tid, c, L = _attn_case(dtype, 40, 1, 8, 2, 128, P, 300, [(13 * i) % 301 for i in range(40)])
@@ -511,6 +526,38 @@ def test_decode_steps_with_a_shared_prefix_and_a_budget(dtype):
                 assert same.all()
     assert evictions >= 3
     assert lib().inferno_device_error(0, 1) == 0
+
+
+def test_first_calls_may_be_captured():
+    """A process whose first calls are made under capture."""
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch, longctx_ref as R
+B, H, d = 40, 4, 128
+q = torch.randn(B, 1, H, d, device="cuda", dtype=torch.bfloat16)
+k, v = (torch.randn(B, 64, 2, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+pk, pv = (torch.randn(300, 2, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+lens = torch.full((B,), 60, dtype=torch.int32, device="cuda")
+scores, pos = torch.zeros(B, 2, 64, device="cuda"), torch.zeros(B, 2, 64, dtype=torch.int32, device="cuda")
+out = torch.empty_like(q)
+a = R.attention_args(30, q, out, lens, k, v, pk, pv, scores)
+e = R.evict_args(30, k, v, scores, pos, lens, lens, scores, pos, lens, budget=32)
+wa, we = R.attention_workspace(a), R.evict_workspace(e)
+at = torch.zeros(B, dtype=torch.int32, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    R.rope(R.rope_args(30, q.view(B, -1), None, None, q.view(B, -1), n_tokens=B, n_heads=H, n_kv_heads=0, head_dim=d,
+                       rope_dim=d, positions=at, theta=1e4))
+    R.attention(a, wa)
+    R.evict(e, we)
+g.replay()
+print("lens", lens.unique().tolist(), "finite", bool(out.isfinite().all()))
+""" % (str(R.__file__).rsplit("/", 1)[0], str(R.InfernoRope.__module__ and __import__("inferno_b200").__path__[0]).rsplit("/", 1)[0])
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert "lens [32] finite True" in out.stdout, out.stdout + out.stderr[-2000:]
 
 
 def test_host_memory_is_refused():
