@@ -291,7 +291,7 @@ typedef struct InfernoEvict {
   int32_t struct_size;
   int32_t type;
   int32_t batch, n_kv_heads, head_dim;
-  int32_t max_len;
+  int32_t max_len;               /* at most 1000000 */
   int32_t budget;                /* >= 1 */
   int32_t n_sink, n_recent;      /* n_sink + n_recent <= budget */
   int32_t reserved;              /* 0 */

@@ -26,12 +26,12 @@ namespace inf {
 
 namespace cg = cooperative_groups;
 
-constexpr int EV_THREADS = 512;
+constexpr int EV_THREADS = 1024;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_MOVE_THREADS = 256;
 constexpr int EV_BINS = 256;
 constexpr int EV_MAX_CLUSTER = 16;         // B200's largest, above the portable 8
-constexpr int EV_MAX_LEN = 1 << 21;         // the bitmaps of a CTA's part fit shared memory up to here
+constexpr int EV_MAX_LEN = 1000000;         // a sixteenth has fewer than 2^16 rows (counts), and its bitmaps fit shared memory
 constexpr int EV_SMEM = 200 * 1024;
 
 struct EvictParams {
@@ -56,12 +56,13 @@ __device__ __forceinline__ uint32_t ev_key(float s) { return s != s ? 0u : float
 
 // what a CTA's peers read
 struct EvShared {
-  int hist[2][EV_BINS];               // counts of a digit
+  uint32_t hist[2][EV_BINS / 2];      // counts of a digit, two 16-bit ones per word: half the bytes to read
   int4 border;                        // ties before / behind the budget, other rows to leave before it / to keep behind it
   int always;                         // rows kept always
   // the CTA's own
-  alignas(16) int total[EV_BINS];     // counts over the cluster
-  int warp_sums[2][EV_WARPS];
+  int2 warp_sums[EV_WARPS], sum;
+  int bin_sums[EV_BINS / 64];
+  int digit, need;
 };
 
 // exclusive sums of x and y over the CTA in thread order; the CTA's in sum_x, sum_y
@@ -73,22 +74,28 @@ __device__ __forceinline__ void ev_scan(EvShared& s, int& x, int& y, int& sum_x,
     const int u = __shfl_up_sync(0xffffffffu, a, o), v = __shfl_up_sync(0xffffffffu, b, o);
     if (lane >= o) a += u, b += v;
   }
+  __syncthreads();                     // the last call's sums are read
+  if (lane == 31) s.warp_sums[warp] = make_int2(a, b);
   __syncthreads();
-  if (lane == 31) s.warp_sums[0][warp] = a, s.warp_sums[1][warp] = b;
-  __syncthreads();
-  int ba = 0, bb = 0;
-  sum_x = sum_y = 0;
+  if (warp == 0) {                     // EV_WARPS = 32
+    const int2 w = s.warp_sums[lane];
+    int c = w.x, d = w.y;
 #pragma unroll
-  for (int w = 0; w < EV_WARPS; ++w) {
-    const int u = s.warp_sums[0][w], v = s.warp_sums[1][w];
-    if (w < warp) ba += u, bb += v;
-    sum_x += u, sum_y += v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, c, o), v = __shfl_up_sync(0xffffffffu, d, o);
+      if (lane >= o) c += u, d += v;
+    }
+    s.warp_sums[lane] = make_int2(c - w.x, d - w.y);
+    if (lane == 31) s.sum = make_int2(c, d);
   }
-  x = ba + a - x;
-  y = bb + b - y;
+  __syncthreads();
+  const int2 base = s.warp_sums[warp], all = s.sum;
+  x = base.x + a - x;
+  y = base.y + b - y;
+  sum_x = all.x, sum_y = all.y;
 }
 
-__global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_constant__ EvictParams p) {
+__global__ void __launch_bounds__(EV_THREADS, 1) evict_kernel(const __grid_constant__ EvictParams p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = cluster.num_blocks(), c = cluster.block_rank();
   const int bh = blockIdx.x / nc, b = bh / p.nkv, h = bh - b * p.nkv;
@@ -124,7 +131,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   const int words_all = (len + 31) >> 5, wpc = (words_all + nc - 1) / nc;
   const int j0 = min(c * wpc, words_all) * 32, n = min(len - j0, wpc * 32), nw = (n + 31) >> 5;
   const int recent_from = (int)max(-2147483648ll, (long long)p.next_pos[b] - p.n_recent);
-  (&sh.hist[0][0])[t] = 0;                    // 2 x 256 bins, 512 threads
+  if (t < EV_BINS) (&sh.hist[0][0])[t] = 0;
   if (t == 0) sh.always = 0;
   __syncthreads();
   auto key_of = [&](int i) { return p.cached ? skey[i] : ev_key(sc[j0 + i]); };
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
       if (lane == 0) always[w] = m;
       n_always += __popc(m);
       if (p.cached) skey[i] = k;
-      if (in && !al) atomicAdd(&sh.hist[0][k >> 24], 1);
+      if (in && !al) atomicAdd(&sh.hist[0][k >> 25], 1u << (k >> 24 & 1) * 16);
     }
   }
   if (lane == 0 && n_always) atomicAdd(&sh.always, n_always);
@@ -166,7 +173,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
       for (int i = t; i < n; i += EV_THREADS) {
         const uint32_t k = key_of(i);
         if ((((always[i >> 5] >> (i & 31)) & 1) != 0) == among_always && (shift == 24 || (k >> (shift + 8)) == prefix))
-          atomicAdd(&sh.hist[buf][(k >> shift) & 255], 1);
+          atomicAdd(&sh.hist[buf][(k >> (shift + 1)) & 127], 1u << (k >> shift & 1) * 16);
       }
     }
     sync_all();
@@ -181,41 +188,44 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
         continue;
       }
     }
-    if (t < EV_BINS) {
-      int x = 0;
+    // thread t: bins 2 t and 2 t + 1 of the whole cluster, and what lies in the bins
+    // above; the digit's bin holds the need-th largest key (need 0: no row of this
+    // class)
+    int lo = 0, hi = 0, above = 0;
+    if (t < EV_BINS / 2) {
+      if (nc == 1) {
+        lo = sh.hist[buf][t] & 0xffff;
+        hi = sh.hist[buf][t] >> 16;
+      } else {
+        uint32_t x[EV_MAX_CLUSTER];           // all loads in flight
 #pragma unroll
-      for (int r = 0; r < EV_MAX_CLUSTER; ++r)
-        if (r < nc) x += cluster.map_shared_rank(&sh.hist[buf][0], r)[t];
-      sh.total[t] = x;
+        for (int r = 0; r < EV_MAX_CLUSTER; ++r) x[r] = r < nc ? cluster.map_shared_rank(&sh.hist[buf][0], r)[t] : 0u;
+#pragma unroll
+        for (int r = 0; r < EV_MAX_CLUSTER; ++r) lo += x[r] & 0xffff, hi += x[r] >> 16;
+      }
       sh.hist[buf ^ 1][t] = 0;                // free: its readers passed the barrier above
+      above = lo + hi;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_down_sync(0xffffffffu, above, o);
+        if (lane + o < 32) above += u;
+      }
+      if (lane == 0) sh.bin_sums[warp] = above;
+    }
+    if (t == EV_BINS) sh.digit = 255, sh.need = 0;
+    __syncthreads();
+    if (t < EV_BINS / 2) {
+      above -= lo + hi;
+#pragma unroll
+      for (int w = 1; w < EV_BINS / 64; ++w)
+        if (w > warp) above += sh.bin_sums[w];
+      if (above < need && above + hi >= need) sh.digit = 2 * t + 1, sh.need = need - above;
+      above += hi;
+      if (above < need && above + lo >= need) sh.digit = 2 * t, sh.need = need - above;
     }
     __syncthreads();
-    // every warp: lane l has bins 8 l .. 8 l + 7; the digit's bin holds the need-th
-    // largest key (need 0: no row of this class, any digit does)
-    int cnt[8], mine = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      const int4 x = *(const int4*)&sh.total[8 * lane + i];
-      cnt[i] = x.x, cnt[i + 1] = x.y, cnt[i + 2] = x.z, cnt[i + 3] = x.w;
-      mine += x.x + x.y + x.z + x.w;
-    }
-    int above = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_down_sync(0xffffffffu, above, o);
-      if (lane + o < 32) above += u;
-    }
-    above -= mine;
-    int digit = -1, rest = 0;
-#pragma unroll
-    for (int i = 7; i >= 0; --i) {
-      if (above < need && above + cnt[i] >= need) digit = 8 * lane + i, rest = need - above;
-      above += cnt[i];
-    }
-    const uint32_t who = __ballot_sync(0xffffffffu, digit >= 0);
-    const int from = who ? __ffs(who) - 1 : 0;
-    digit = who ? __shfl_sync(0xffffffffu, digit, from) : 255;
-    need = who ? __shfl_sync(0xffffffffu, rest, from) : 0;
+    const int digit = sh.digit;
+    need = sh.need;
     prefix = (prefix << 8) | (uint32_t)digit;
     buf ^= 1;
     shift -= 8;
@@ -238,17 +248,17 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
     const int m = p.budget - (j0 + w * 32);
     return m >= 32 ? 0xffffffffu : m <= 0 ? 0u : (1u << m) - 1;
   };
-  int ties = 0, ties_front = 0, sum, sum_front;
-  int leave = 0, stay = 0, sum_leave, sum_stay;
+  // counts of a part fit 16 bits: two per scanned word
+  int tf = 0, ls = 0, sum_tf, sum_ls;        // ties, and those in front; leave in front, stay behind
   for (int w = w_lo; w < w_hi; ++w) {
     const uint32_t f = front(w);
-    ties += __popc(tie[w]);
-    ties_front += __popc(tie[w] & f);
-    leave += __popc(~(keep[w] | tie[w]) & valid(w) & f);
-    stay += __popc(keep[w] & ~f);
+    tf += __popc(tie[w]) | __popc(tie[w] & f) << 16;
+    ls += __popc(~(keep[w] | tie[w]) & valid(w) & f) | __popc(keep[w] & ~f) << 16;
   }
-  ev_scan(sh, ties, ties_front, sum, sum_front);
-  ev_scan(sh, leave, stay, sum_leave, sum_stay);
+  ev_scan(sh, tf, ls, sum_tf, sum_ls);
+  int ties = tf & 0xffff;
+  const int sum = sum_tf & 0xffff, sum_front = (uint32_t)sum_tf >> 16;
+  const int sum_leave = sum_ls & 0xffff, sum_stay = (uint32_t)sum_ls >> 16;
   if (t == 0) sh.border = make_int4(sum_front, sum - sum_front, sum_leave, sum_stay);
   sync_all();
   // lane r: CTA r's part.  Its ties are kept as far as `need` reaches after those
@@ -279,7 +289,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
     nh += base_h[w] = __popc(~k & valid(w) & front(w));
     ns += base_s[w] = __popc(k & ~front(w));
   }
-  ev_scan(sh, nh, ns, sum, sum_front);
+  int sum_h, sum_s;
+  ev_scan(sh, nh, ns, sum_h, sum_s);
   holes += nh, srcs += ns;
   for (int w = w_lo; w < w_hi; ++w) {
     const int x = base_h[w], y = base_s[w];
@@ -477,15 +488,15 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.max_moves = evict_max_moves(e);
   p.lists = (int*)workspace;
   if (e->lens_out == e->lens) p.lens_out = nullptr;
-  // CTAs per (sequence, KV head), up to 16 and while all run at once, two per SM: one
-  // per 1024 rows to rank (4160 rows in 32 heads: 17.7 us with four, 20.6 with one,
-  // which waits for itself instead of the others) or per 256 KB to move
+  // CTAs per (sequence, KV head), up to 16 and while all run at once: one per 4096
+  // rows to rank (fewer do not pay for the cluster's barriers, of which one CTA has
+  // none) or per 512 KB to move
   const int n = e->batch * e->n_kv_heads;
   int dev = 0;
   INF_CUDA_TRY(cudaGetDevice(&dev));
   int nc = 1;
-  while (nc < EV_MAX_CLUSTER && n * nc * 2 <= 2 * num_sms(dev) &&
-         (e->max_len >= nc * 2 * 1024 || 4ll * p.max_moves * p.head_bytes >= nc * 2 * (256ll << 10)))
+  while (nc < EV_MAX_CLUSTER && n * nc * 2 <= num_sms(dev) &&
+         (e->max_len >= nc * 2 * 4096 || 4ll * p.max_moves * p.head_bytes >= nc * 2 * (512ll << 10)))
     nc *= 2;
   auto smem_of = [&](int ctas, bool cached) {
     const long long words = ((e->max_len + 31) / 32 + ctas - 1) / ctas;
@@ -495,10 +506,10 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.cached = smem_of(nc, true) <= EV_SMEM;
   p.words = ((e->max_len + 31) / 32 + nc - 1) / nc;
   const size_t smem = smem_of(nc, p.cached);
-  // fewer than one CTA per SM and more than 1 MB to move: a second kernel over the
-  // whole GPU moves K and V (4 heads of 62898 fp32 rows of 128 to 14946: 105 us
-  // with the 32 CTAs alone)
-  const bool spread = n * nc < num_sms(dev) && 4ll * p.max_moves * p.head_bytes * n > (1 << 20);
+  // much to move by less than half of the SMs: a second kernel over the whole GPU
+  // moves K and V (4 heads of 62898 fp32 rows of 128 to 14946: 105 us with 32 CTAs
+  // alone, 45 with it)
+  const bool spread = n * nc * 2 < num_sms(dev) && 4ll * p.max_moves * p.head_bytes > nc * (512ll << 10);
   if (spread) p.counts = (int*)workspace + (long long)n * 2 * p.max_moves;
   cudaStream_t st = (cudaStream_t)stream;
   static DeviceOnce once;

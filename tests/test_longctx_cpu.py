@@ -111,7 +111,7 @@ def test_attention_workspace_checked():
 
 EVICT_SIZES = [
     (dict(type=12), "type"), (dict(batch=-1), "sizes"), (dict(n_kv_heads=0), "sizes"), (dict(batch=40000), "sizes"),
-    (dict(max_len=-1), "sizes"), (dict(head_dim=65), "head_dim"), (dict(head_dim=16384), "head_dim"),
+    (dict(max_len=-1), "sizes"), (dict(max_len=1000001, seq_stride=1 << 40, score_stride=1 << 30), "max_len"), (dict(head_dim=65), "head_dim"), (dict(head_dim=16384), "head_dim"),
     (dict(budget=0), "budget"), (dict(n_sink=17), "budget"), (dict(n_recent=-1), "budget"), (dict(reserved=1), "reserved"),
 ]
 
