@@ -7,7 +7,8 @@
 // (n_tokens x group for its own rows, batch x n_tokens x group for the prefix).
 //
 // ac_part_kernel: a CTA takes 16 R query rows of one KV head (prefix: of all
-// sequences; own part: of one) against one split of the keys.  Its warps form NG
+// sequences; own part: of one) against a range of keys (attn_cached.h says how they
+// are cut).  Its warps form NG
 // key groups of R warps; each group walks its own tiles of 16 keys with a ring of
 // cp.async slots (a K or a V tile per slot, rows past the end zero-filled), each
 // warp holds 16 rows: S = Q K^T and O += P V by mma.sync with the running
@@ -17,7 +18,7 @@
 // about 21 significant bits.  The groups merge in shared memory.
 // ac_vec_kernel: the same for fp32 and few query rows, on the CUDA cores, a lane
 // holding some dims of the rows and of the keys (see there).
-// ac_finish_kernel: joins the splits of a row, and adds the weights of the own
+// ac_finish_kernel: joins the partial results of a row, and adds the weights of the own
 // rows to `scores` from the logits that the first kernel left.
 #include <algorithm>
 #include <cmath>
@@ -33,6 +34,7 @@ namespace inf {
 
 namespace {
 
+constexpr int AC_SMS = 148;                     // of a B200
 constexpr int AC_KT = 16;                       // keys per tile
 constexpr int AC_SMEM = 227 * 1024, AC_SMEM_HALF = 112 * 1024;
 constexpr int AC_FIN_THREADS = 256;
@@ -300,27 +302,18 @@ __device__ __forceinline__ long long ac_entry(const AcParams& p, const AcWork& w
   return ((long long)(b * p.n_tok + t) * p.nh + h) * p.p_splits + w.split;
 }
 
+// one piece of work of a CTA, from its first copies to its partial results
 template <typename T, int HD, int R>
-__global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTAS) ac_part_kernel(const __grid_constant__ AcParams p, AcGrid gr) {
+__device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork w, uint8_t* smem) {
   using G = AcGeo<T, HD, R>;
   constexpr bool F32 = AcType<T>::F32;
   constexpr int ROW = G::ROW, ITEM = G::ITEM, SLOTS = G::SLOTS, GT = R * 32;
-  extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int grp = warp / R, rt = warp - grp * R;       // key group, row tile of the warp
   const int gtid = tid - grp * GT;                     // thread within the group
-
-  __shared__ AcCursor s_cur;
-  __shared__ AcWork s_work;
-  pdl_trigger();
-  if (warp == 0) ac_first<T, HD>(p, gr, 16 * R, s_cur, s_work);
-  for (;;) {
-  __syncthreads();
-  const AcWork w = s_work;
-  if (w.j0 >= w.j1) break;
   const long long key_stride = (long long)p.nkv * ROW;
 
-  const uint32_t s_q = smem_u32(smem);                            // fp32 only: [16 R][HD]
+  const uint32_t s_q = smem_u32(smem);                            // with QS: [16 R][HD]
   uint8_t* ring_p = smem + G::QBYTES;
   const uint32_t ring = smem_u32(ring_p) + grp * SLOTS * ITEM;
   float2* s_ml = (float2*)(smem + G::BODY);                      // [NW][16]
@@ -681,8 +674,22 @@ __global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTA
       p.part_ml[at] = make_float2(M, L);
     }
   }
-  __syncthreads();                     // the merge buffer is the next segment's ring
-  if (tid == 0) ac_next<T, HD>(p, s_cur, s_work);
+}
+
+template <typename T, int HD, int R>
+__global__ void __launch_bounds__(AcGeo<T, HD, R>::THREADS, AcGeo<T, HD, R>::CTAS) ac_part_kernel(const __grid_constant__ AcParams p, AcGrid gr) {
+  extern __shared__ __align__(128) uint8_t ac_smem[];
+  __shared__ AcCursor s_cur;
+  __shared__ AcWork s_work;
+  pdl_trigger();
+  if (threadIdx.x < 32) ac_first<T, HD>(p, gr, 16 * R, s_cur, s_work);
+  for (;;) {
+    __syncthreads();
+    const AcWork w = s_work;
+    if (w.j0 >= w.j1) break;
+    ac_part_segment<T, HD, R>(p, w, ac_smem);
+    __syncthreads();                   // the merge buffer is the next segment's ring
+    if (threadIdx.x == 0) ac_next<T, HD>(p, s_cur, s_work);
   }
   // launched beside the prefix part: not complete before it, so that the
   // finishing kernel, which waits for this one, finds both
@@ -711,21 +718,17 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 template <int HD, int RN>
-__global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kernel(const __grid_constant__ AcParams p, AcGrid gr) {
+struct AvShared {
+  float merge[AV_WARPS][RN][HD];
+  float2 ml[AV_WARPS][RN];
+  float q[RN][HD];
+};
+
+template <int HD, int RN>
+__device__ __forceinline__ void ac_vec_segment(const AcParams& p, const AcWork w, AvShared<HD, RN>& sh) {
   constexpr int KT = 32 / RN;                      // keys of a tile
   constexpr int D2 = HD / 64;                      // float2 of a lane
-  __shared__ float merge[AV_WARPS][RN][HD];
-  __shared__ float2 s_ml[AV_WARPS][RN];
-  __shared__ float s_q[RN][HD];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_trigger();
-  __shared__ AcCursor s_cur;
-  __shared__ AcWork s_work;
-  if (warp == 0) ac_first<float, HD>(p, gr, RN, s_cur, s_work);
-  for (;;) {
-  __syncthreads();
-  const AcWork w = s_work;
-  if (w.j0 >= w.j1) break;
   const long long key_stride = (long long)p.nkv * HD;
   // dims of float2 i of this lane: pairs (0, 1) and (2, 3) are one 16-byte access
   auto dim = [&](int i) { return 128 * (i >> 1) + 4 * lane + 2 * (i & 1); };
@@ -757,7 +760,7 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
       ac_row(p, w, w.row0 + r, b, t, h);
       x = *(const float4*)((const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD + 4 * c);
     }
-    *(float4*)&s_q[r][4 * c] = x;
+    *(float4*)&sh.q[r][4 * c] = x;
   }
   __syncthreads();
   float2 o[RN][D2];
@@ -783,7 +786,7 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
 #pragma unroll
     for (int r = 0; r < RN; ++r) {
       float2 q[D2];
-      load(s_q[r], true, q);
+      load(sh.q[r], true, q);
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
         float2 a = make_float2(0.f, 0.f);
@@ -850,16 +853,16 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
   // ---- merge the warps ----
 #pragma unroll
   for (int of = RN; of < 32; of <<= 1) l += __shfl_xor_sync(0xffffffffu, l, of);
-  if (lane < RN) s_ml[warp][lane] = make_float2(m, l);
+  if (lane < RN) sh.ml[warp][lane] = make_float2(m, l);
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < RN; ++r) {
     float M = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < AV_WARPS; ++x) M = fmaxf(M, s_ml[x][r].x);
-    const float f = ac_weight(s_ml[warp][r], M);
+    for (int x = 0; x < AV_WARPS; ++x) M = fmaxf(M, sh.ml[x][r].x);
+    const float f = ac_weight(sh.ml[warp][r], M);
 #pragma unroll
-    for (int i = 0; i < D2; ++i) *(float2*)&merge[warp][r][dim(i)] = make_float2(o[r][i].x * f, o[r][i].y * f);
+    for (int i = 0; i < D2; ++i) *(float2*)&sh.merge[warp][r][dim(i)] = make_float2(o[r][i].x * f, o[r][i].y * f);
   }
   __syncthreads();
   const int live = min(RN, w.nrows - w.row0);
@@ -868,7 +871,7 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int x = 0; x < AV_WARPS; ++x) {
-      const float4 y = *(const float4*)&merge[x][r][4 * c];
+      const float4 y = *(const float4*)&sh.merge[x][r][4 * c];
       a.x += y.x, a.y += y.y, a.z += y.z, a.w += y.w;
     }
     const long long at = ac_entry(p, w, r);
@@ -876,14 +879,28 @@ __global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kerne
     if (c == 0) {
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int x = 0; x < AV_WARPS; ++x) M = fmaxf(M, s_ml[x][r].x);
+      for (int x = 0; x < AV_WARPS; ++x) M = fmaxf(M, sh.ml[x][r].x);
 #pragma unroll
-      for (int x = 0; x < AV_WARPS; ++x) L += s_ml[x][r].y * ac_weight(s_ml[x][r], M);
+      for (int x = 0; x < AV_WARPS; ++x) L += sh.ml[x][r].y * ac_weight(sh.ml[x][r], M);
       p.part_ml[at] = make_float2(M, L);
     }
   }
-  __syncthreads();
-  if (tid == 0) ac_next<float, HD>(p, s_cur, s_work);
+}
+
+template <int HD, int RN>
+__global__ void __launch_bounds__(AV_WARPS * 32, HD == 256 ? 2 : 3) ac_vec_kernel(const __grid_constant__ AcParams p, AcGrid gr) {
+  __shared__ AvShared<HD, RN> sh;
+  __shared__ AcCursor s_cur;
+  __shared__ AcWork s_work;
+  pdl_trigger();
+  if (threadIdx.x < 32) ac_first<float, HD>(p, gr, RN, s_cur, s_work);
+  for (;;) {
+    __syncthreads();
+    const AcWork w = s_work;
+    if (w.j0 >= w.j1) break;
+    ac_vec_segment<HD, RN>(p, w, sh);
+    __syncthreads();
+    if (threadIdx.x == 0) ac_next<float, HD>(p, s_cur, s_work);
   }
   pdl_wait();                          // see ac_part_kernel
 }
@@ -1106,7 +1123,7 @@ void ac_split(long long units, long long len, int* splits, int* split_len) {
     const long long want = std::max(1ll, std::min(256ll, ctas / units));
     return ((len + want - 1) / want + 63) / 64 * 64;
   };
-  const long long sl = std::max(keys(4 * 296), std::min(256ll, keys(296)));
+  const long long sl = std::max(keys(8 * AC_SMS), std::min(256ll, keys(2 * AC_SMS)));
   *split_len = (int)sl;
   *splits = (int)((len + sl - 1) / sl);
 }
@@ -1178,7 +1195,7 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
     // one round of CTAs: splits of at least two tiles
     pl.p_tiles = (int)((pre + ap_rows() - 1) / ap_rows());
     const long long units = (long long)pl.p_tiles * a->n_kv_heads;
-    const long long want = std::max(1ll, std::min(256ll, 148ll * ap_ctas_per_sm(a->head_dim) / units));
+    const long long want = std::max(1ll, std::min(256ll, (long long)AC_SMS * ap_ctas_per_sm(a->head_dim) / units));
     const long long sl = ((a->prefix_len + want - 1) / want + 63) / 64 * 64;
     p->p_split_len = (int)std::max(128ll, sl);
     p->p_splits = (a->prefix_len + p->p_split_len - 1) / p->p_split_len;
@@ -1193,7 +1210,7 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   // three; two f32 ones of 65536, 28 blocks: 116 in one and 132 in three).
   const long long units = (long long)a->n_kv_heads * p->o_tiles;
   const long long blocks = (long long)a->batch * ((a->max_len + AC_BLOCK - 1) / AC_BLOCK);
-  const long long at_once = 148ll * ac_ctas_per_sm(a->type, a->head_dim, pl.o_r);
+  const long long at_once = (long long)AC_SMS * ac_ctas_per_sm(a->type, a->head_dim, pl.o_r);
   long long groups = units <= at_once / 8 ? at_once / units : (2 * at_once + units - 1) / units;
   groups *= std::max(1ll, std::min(4ll, blocks / (32 * groups)));
   p->o_groups = (int)std::min(blocks, groups);
@@ -1282,7 +1299,7 @@ cudaError_t ac_run(const AcParams& p, const AcPlan& pl, cudaStream_t st) {
   const long long row_blocks = (pl.rows + per_block - 1) / per_block;
   // four cache rows per thread, or one where that leaves fewer than two CTAs per SM
   const long long heads = (long long)p.batch * p.nkv;
-  const int slots = p.scores && heads * ((p.max_len + 4 * AC_FIN_THREADS - 1) / (4 * AC_FIN_THREADS)) >= 296 ? 4 : 1;
+  const int slots = p.scores && heads * ((p.max_len + 4 * AC_FIN_THREADS - 1) / (4 * AC_FIN_THREADS)) >= 2 * AC_SMS ? 4 : 1;
   const long long slot_blocks = p.scores ? (p.max_len + slots * AC_FIN_THREADS - 1) / (slots * AC_FIN_THREADS) : 0;
   const long long blocks = row_blocks + slot_blocks * heads;
   auto* kernel = slots == 4 ? (warps == 1 ? ac_finish_kernel<T, HD, 1, 4> : warps == 4 ? ac_finish_kernel<T, HD, 4, 4> : ac_finish_kernel<T, HD, 8, 4>)
