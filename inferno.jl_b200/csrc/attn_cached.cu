@@ -1139,8 +1139,19 @@ int ac_ctas_per_sm(int type, int hd, int r) {
   return hd == 64 ? ac_ctas_per_sm<__half, 64>(r) : hd == 128 ? ac_ctas_per_sm<__half, 128>(r) : ac_ctas_per_sm<__half, 256>(r);
 }
 
-// The prefix part on tcgen05: 16-bit types with more rows than two tiles of 16
-bool ac_prefix_tc(int type, long long rows) { return type != INFERNO_F32 && rows > 32; }
+// The prefix part of a 16-bit type on tcgen05 or on mma.sync, by the number of
+// products (rows in tiles of 16 x keys x KV heads x head_dim).  tcgen05 streams
+// faster and takes 128 rows at a time, but starts later (TMEM, barriers) and at
+// head_dim 64 waits for its exponentials.  Measured, whole calls, tcgen05 / mma:
+// head_dim 128: 4 rows x 32000 x 8 heads 35 / 41 us, 32 rows 39 / 59; 16 x 16000 x 2
+// 17 / 14; 128 x 500 x 4 12.4 / 13.6; 48 x 300 x 4 12.0 / 11.4; 256: 32 x 8000 x 4 23 /
+// 27, 16 rows 22 / 20; 48 x 300 x 4 14 / 18; 64: 64 x 4000 x 8 17 / 16, 48 x 2000 x 4
+// 12 / 10.
+bool ac_prefix_tc(const InfernoAttention* a, long long rows) {
+  if (a->type == INFERNO_F32) return false;
+  const double products = (double)((rows + 15) / 16 * 16) * a->prefix_len * a->n_kv_heads * a->head_dim;
+  return products >= (a->head_dim == 64 ? 256e6 : rows > 32 ? 10e6 : 200e6);
+}
 
 int ac_check(const InfernoAttention* a) {
   if (!a) return set_error(INFERNO_EINVAL, "attention_cached: null parameters");
@@ -1182,14 +1193,14 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   pl.p_r = ac_row_class(a->type, a->head_dim, pre, a->prefix_len);
   // both parts in one launch where the own part is small beside the prefix and
   // can take the prefix part's kernel: a launch costs more than idle rows then
-  if (a->prefix_len && a->max_len && pl.p_r > pl.o_r && (pl.p_r <= 8 || pl.o_r >= 16) && !ac_prefix_tc(a->type, pre) &&
+  if (a->prefix_len && a->max_len && pl.p_r > pl.o_r && (pl.p_r <= 8 || pl.o_r >= 16) && !ac_prefix_tc(a, pre) &&
       (long long)a->max_len * a->batch <= a->prefix_len)
     pl.o_r = pl.p_r;
   p->o_rows = pl.o_r;
   p->o_tiles = (int)((own + pl.o_r - 1) / pl.o_r);
   pl.p_tiles = (int)((pre + pl.p_r - 1) / pl.p_r);
   p->p_splits = 0;
-  pl.p_tc = ac_prefix_tc(a->type, pre);
+  pl.p_tc = ac_prefix_tc(a, pre);
   if (!a->prefix_len) {
   } else if (pl.p_tc) {
     // one round of CTAs: splits of at least two tiles

@@ -96,6 +96,7 @@ __device__ __forceinline__ void ev_scan(EvShared& s, int& x, int& y, int& sum_x,
 }
 
 __global__ void __launch_bounds__(EV_THREADS, 1) evict_kernel(const __grid_constant__ EvictParams p) {
+  pdl_trigger();                              // evict_move_kernel may take its places on the idle SMs
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = cluster.num_blocks(), c = cluster.block_rank();
   const int bh = blockIdx.x / nc, b = bh / p.nkv, h = bh - b * p.nkv;
@@ -488,14 +489,17 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   p.max_moves = evict_max_moves(e);
   p.lists = (int*)workspace;
   if (e->lens_out == e->lens) p.lens_out = nullptr;
-  // CTAs per (sequence, KV head), up to 16 and while all run at once: one per 4096
-  // rows to rank (fewer do not pay for the cluster's barriers, of which one CTA has
-  // none) or per 512 KB to move
+  // CTAs per (sequence, KV head), up to 16: one per 4096 rows to rank (fewer do not
+  // pay for the cluster's barriers, of which one CTA has none) or per 512 KB to move.
+  // All clusters have to run at once, an SM per CTA (a second round of them costs a
+  // whole ranking): 35 clusters of 4 fit, 16 of 8 and 7 of 16 at best, so clusters of
+  // 8 and 16 are kept to 64 CTAs (8 heads of 54775 fp32 rows: 39 us with 8 CTAs each,
+  // 65 with 16)
   const int n = e->batch * e->n_kv_heads;
   int dev = 0;
   INF_CUDA_TRY(cudaGetDevice(&dev));
   int nc = 1;
-  while (nc < EV_MAX_CLUSTER && n * nc * 2 <= num_sms(dev) &&
+  while (nc < EV_MAX_CLUSTER && n * nc * 2 <= (nc >= 4 ? 64 : 128) &&
          (e->max_len >= nc * 2 * 4096 || 4ll * p.max_moves * p.head_bytes >= nc * 2 * (512ll << 10)))
     nc *= 2;
   auto smem_of = [&](int ctas, bool cached) {
@@ -532,7 +536,7 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
     err = cudaLaunchKernelEx(&cfg, evict_kernel, p);
   }
   if (err == cudaSuccess && (spread || !p.lens_out)) {
-    const int rows = std::max(1, (32 << 10) / p.head_bytes);         // 64 KB of K and V per block
+    const int rows = std::max(1, (16 << 10) / p.head_bytes);         // 32 KB of K and V: one piece in flight each
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(spread ? (p.max_moves + rows - 1) / rows : 1), (unsigned)n);
     cfg.blockDim = dim3(EV_MOVE_THREADS);

@@ -224,6 +224,9 @@ ATTN = [
     ("bf16", 3, 1, 4, 4, 128, 257, 50, [60, -3, 50]),                # lens outside [0, max_len] are clamped
     ("f16", 2, 1, 16, 1, 256, 4097, 100, [100, 99]),
     ("bf16", 17, 8, 8, 1, 64, 1, 9, [9] * 17),
+    ("f16", 1, 1, 16, 4, 128, 40001, 5, [5]),                        # four query rows on a long prefix
+    ("bf16", 3, 1, 12, 4, 64, 100001, 5, [5, 1, 0]),
+    ("bf16", 65, 1, 16, 4, 64, 4097, 3, [3] * 65),                   # 260 prefix rows, the last four in a tile of their own
 ]
 
 
@@ -276,12 +279,14 @@ def test_attention_extremes(dtype):
     _check_attn(tid, c, L)
 
 
-@pytest.mark.parametrize("dtype,kv,d,scale", [("bf16", 1, 128, 0.0), ("f16", 2, 64, -0.4), ("bf16", 1, 256, 0.1)])
-def test_attention_prefix_maximum_rises(dtype, kv, d, scale):
+@pytest.mark.parametrize("dtype,kv,d,scale,P", [("bf16", 1, 128, 0.0, 3000), ("f16", 2, 64, -0.4, 3000),
+                                                ("bf16", 1, 256, 0.1, 3000), ("f16", 4, 64, 0.0, 6001),
+                                                ("bf16", 4, 64, -0.2, 6017)])
+def test_attention_prefix_maximum_rises(dtype, kv, d, scale, P):
     """Many query rows on a prefix whose logits grow along it, so that the running
     maximum rises by far more than the slack again and again, in some rows only."""
-    tid, c, L = _attn_case(dtype, 24, 2, 4 * kv, kv, d, 3000, 40, [40 - b for b in range(24)])
-    c["pk"] *= torch.linspace(0.05, 6, 3000, device="cuda")[:, None, None].to(c["pk"].dtype)
+    tid, c, L = _attn_case(dtype, 24, 2, 4 * kv, kv, d, P, 40, [40 - b for b in range(24)])
+    c["pk"] *= torch.linspace(0.05, 6, P, device="cuda")[:, None, None].to(c["pk"].dtype)
     c["q"][::3] *= 0.01
     _check_attn(tid, c, L, scale)
     assert lib().inferno_device_error(0, 0) == 0
@@ -539,7 +544,7 @@ import torch, longctx_ref as R
 B, H, d = 40, 4, 128
 q = torch.randn(B, 1, H, d, device="cuda", dtype=torch.bfloat16)
 k, v = (torch.randn(B, 64, 2, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
-pk, pv = (torch.randn(300, 2, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+pk, pv = (torch.randn(1000, 2, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
 lens = torch.full((B,), 60, dtype=torch.int32, device="cuda")
 scores, pos = torch.zeros(B, 2, 64, device="cuda"), torch.zeros(B, 2, 64, dtype=torch.int32, device="cuda")
 out = torch.empty_like(q)
