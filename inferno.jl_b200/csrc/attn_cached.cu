@@ -1330,6 +1330,7 @@ using namespace inf;
 extern "C" int64_t inferno_attention_cached_workspace(const InfernoAttention* a) {
   const int rc = ac_check(a);
   if (rc) return rc;
+  if (a->batch == 0) return 256;              // nothing to plan for
   AcParams p{};
   return (int64_t)ac_plan(a, &p).bytes;
 }

@@ -3,6 +3,7 @@ bad argument is turned into a status and a message before any device work."""
 import ctypes as C
 import shutil
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -127,6 +128,19 @@ def test_evict_refuses(kw, word):
 @pytest.mark.parametrize("kw,word", EVICT_SIZES)
 def test_evict_workspace_refuses(kw, word):
     _refused(lib().inferno_cache_evict_workspace(C.byref(_evict(**kw))), word)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(type=0, head_dim=256), dict(prefix_len=0), dict(prefix_len=1 << 20),
+                                dict(n_tokens=1 << 30, n_heads=8, n_kv_heads=2)])
+def test_attention_workspace_of_an_empty_batch(kw):
+    # a status or a size: an empty batch has no rows to cut the prefix for
+    code = ("import ctypes as C\n"
+            "from inferno_b200._lib import InfernoAttention, lib\n"
+            f"a = InfernoAttention(**{dict(dict(type=30, batch=0, n_tokens=1, n_heads=8, n_kv_heads=2, head_dim=64, prefix_len=100, max_len=50), **kw)!r})\n"
+            "print(lib().inferno_attention_cached_workspace(C.byref(a)))\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                       cwd=HEADER.parent.parent / "inferno.jl_b200", timeout=120)
+    assert r.returncode == 0 and int(r.stdout) >= 0, (r.returncode, r.stderr)
 
 
 def test_evict_workspace_checked():
