@@ -5,10 +5,11 @@
 // integer, in two classes (rows kept always come first); it is read once into
 // shared memory.  The budget-th largest key is found by a radix select of four
 // 8-bit digits: every CTA counts its own rows, reads the others' counts through
-// distributed shared memory and finds the digit for itself.  (Digits of 11 bits
+// distributed shared memory and finds the digit for itself; it ends early where all
+// rows of the border's bin stay.  (Digits of 11 bits
 // save a barrier and cost eight times the remote reads, which are what a pass
 // waits for: 10 us a pass measured with 8 CTAs, 1 us with 8 bits.)
-// Ties at that key go to the lowest rows.  Which rows stay is then a bitmap, so
+// Ties at that key (or in that bin) go to the lowest rows.  Which rows stay is then a bitmap, so
 // ranks are bit counts: the i-th kept row behind the budget goes into the i-th
 // hole before it.  The two lists have equal lengths and no row is both read and
 // written, so the CTAs of the cluster move K and V in any order.
@@ -62,7 +63,7 @@ struct EvShared {
   // the CTA's own
   int2 warp_sums[EV_WARPS], sum;
   int bin_sums[EV_BINS / 64];
-  int digit, need;
+  int digit, need, in_bin;             // in_bin: rows in the digit's bin
 };
 
 // exclusive sums of x and y over the CTA in thread order; the CTA's in sum_x, sum_y
@@ -104,13 +105,13 @@ __global__ void __launch_bounds__(EV_THREADS, 1) evict_kernel(const __grid_const
   __shared__ EvShared sh;
   extern __shared__ uint32_t ev_dyn[];
   uint32_t* always = ev_dyn;                  // bit per row of the part: kept always
-  uint32_t* tie = always + p.words;           // key equal to the border
+  uint32_t* tie = always + p.words;           // key equal to the border in its leading digits
   uint32_t* keep = tie + p.words;
   int* base_h = (int*)(keep + p.words);       // holes / sources before a word
   int* base_s = base_h + p.words;
   uint32_t* skey = (uint32_t*)(base_s + p.words);
 
-  const int len = max(0, min(p.lens[b], p.max_len));
+  const int next = p.next_pos[b], len = max(0, min(p.lens[b], p.max_len));
   if (p.lens_out && h == 0 && c == 0 && t == 0) p.lens_out[b] = min(len, p.budget);
   const float* sc = p.scores + bh * p.stride;
   const int* ps = p.pos + bh * p.stride;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) evict_kernel(const __grid_const
   // this CTA's rows [j0, j0 + n), in words of 32
   const int words_all = (len + 31) >> 5, wpc = (words_all + nc - 1) / nc;
   const int j0 = min(c * wpc, words_all) * 32, n = min(len - j0, wpc * 32), nw = (n + 31) >> 5;
-  const int recent_from = (int)max(-2147483648ll, (long long)p.next_pos[b] - p.n_recent);
+  const int recent_from = (int)max(-2147483648ll, (long long)next - p.n_recent);
   if (t < EV_BINS) (&sh.hist[0][0])[t] = 0;
   if (t == 0) sh.always = 0;
   __syncthreads();
@@ -167,9 +168,9 @@ __global__ void __launch_bounds__(EV_THREADS, 1) evict_kernel(const __grid_const
   // the class the border lies in: the others, or the rows kept always should they
   // exceed the budget (the first digit is then counted again)
   bool among_always = false, recount = false;
-  int need = 0, buf = 0;
+  int need = 0, buf = 0, shift = 24;
   uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0;) {
+  while (shift >= 0) {
     if (shift < 24 || recount) {
       for (int i = t; i < n; i += EV_THREADS) {
         const uint32_t k = key_of(i);
@@ -213,16 +214,16 @@ __global__ void __launch_bounds__(EV_THREADS, 1) evict_kernel(const __grid_const
       }
       if (lane == 0) sh.bin_sums[warp] = above;
     }
-    if (t == EV_BINS) sh.digit = 255, sh.need = 0;
+    if (t == EV_BINS) sh.digit = 255, sh.need = sh.in_bin = 0;
     __syncthreads();
     if (t < EV_BINS / 2) {
       above -= lo + hi;
 #pragma unroll
       for (int w = 1; w < EV_BINS / 64; ++w)
         if (w > warp) above += sh.bin_sums[w];
-      if (above < need && above + hi >= need) sh.digit = 2 * t + 1, sh.need = need - above;
+      if (above < need && above + hi >= need) sh.digit = 2 * t + 1, sh.need = need - above, sh.in_bin = hi;
       above += hi;
-      if (above < need && above + lo >= need) sh.digit = 2 * t, sh.need = need - above;
+      if (above < need && above + lo >= need) sh.digit = 2 * t, sh.need = need - above, sh.in_bin = lo;
     }
     __syncthreads();
     const int digit = sh.digit;
@@ -230,15 +231,17 @@ __global__ void __launch_bounds__(EV_THREADS, 1) evict_kernel(const __grid_const
     prefix = (prefix << 8) | (uint32_t)digit;
     buf ^= 1;
     shift -= 8;
+    if (sh.in_bin == need) break;             // all of the bin: the digits below do not matter (mostly the last one)
   }
+  const int low = shift + 8;                  // bits of the digits left out
 
   // ---- bitmaps: kept for certain, and ties at the border ------------------------------
   for (int w = warp; w < nw; w += EV_WARPS) {
     const int i = w * 32 + lane;
     const uint32_t k = i < n ? key_of(i) : 0u;
     const bool al = (always[w] >> lane) & 1, in_class = i < n && al == among_always;
-    const uint32_t m_tie = __ballot_sync(0xffffffffu, in_class && k == prefix);
-    const uint32_t m_keep = __ballot_sync(0xffffffffu, i < n && (in_class ? k > prefix : al));
+    const uint32_t m_tie = __ballot_sync(0xffffffffu, in_class && k >> low == prefix);
+    const uint32_t m_keep = __ballot_sync(0xffffffffu, i < n && (in_class ? k >> low > prefix : al));
     if (lane == 0) tie[w] = m_tie, keep[w] = m_keep;
   }
   __syncthreads();

@@ -440,6 +440,25 @@ def test_evict_ties_and_odd_scores(kind):
     _check_evict(tid, k, v, scores, pos, [2500, 2049], [2500, 2500], budget=1300, n_sink=3, n_recent=50)
 
 
+@pytest.mark.parametrize("rows", [2000, 20000])
+@pytest.mark.parametrize("bit", [0, 7, 8, 15, 16, 22, 23, 26, 31])
+@pytest.mark.parametrize("short", [0, 1, -1])
+def test_evict_border_between_two_values(rows, bit, short):
+    """Scores of two values that differ in one bit, as many of the larger as the
+    budget holds, one more and one fewer."""
+    tid, k, v, scores, pos = _evict_case("f16", 1, 2, 8, rows, seed=bit)
+    hi = rows // 3
+    low = 0x3a000000
+    bits = torch.full(scores.shape, low, dtype=torch.int64, device="cuda")
+    for h in range(2):
+        at = torch.randperm(rows, generator=_gen(bit + 40 + h), device="cuda")[:hi]
+        bits[0, h, at] = low ^ (1 << bit)
+    if bit == 31 or low & (1 << bit):          # the changed value is the smaller one
+        hi = rows - hi
+    scores.copy_(torch.where(bits >= 2**31, bits - 2**32, bits).to(torch.int32).view(torch.float32))
+    _check_evict(tid, k, v, scores, pos, [rows], [rows], budget=hi + short, n_sink=0, n_recent=0)
+
+
 def test_evict_more_kept_always_than_budget():
     """Positions named twice can put more rows under protection than the budget
     holds: they are then ranked by score."""
