@@ -1114,18 +1114,25 @@ int ac_row_class(int type, int hd, long long rows, int len) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
-// Splits of the prefix when `units` (KV heads x row tiles) share the GPU: about four
-// rounds of two CTAs per SM as long as a split keeps 256 keys (below that starting
-// and merging a CTA costs more than it streams); with fewer keys, one round, down
-// to 64 keys, one tile of 16 for each of four key groups.
-void ac_split(long long units, long long len, int* splits, int* split_len) {
-  auto keys = [&](long long ctas) {
-    const long long want = std::max(1ll, std::min(256ll, ctas / units));
-    return ((len + want - 1) / want + 63) / 64 * 64;
-  };
-  const long long sl = std::max(keys(8 * AC_SMS), std::min(256ll, keys(2 * AC_SMS)));
-  *split_len = (int)sl;
-  *splits = (int)((len + sl - 1) / sl);
+// Splits of the prefix when `units` (KV heads x row tiles) share the GPU, of which
+// at_once CTAs run at a time: as many as fill one to four rounds of CTAs, whichever
+// ends first when a CTA takes the time of its keys and of `start` more.  (Against
+// splits of 256 keys in any number of rounds, fp32: 32 query rows of head_dim 256 x 4
+// heads on 16000 keys, 252 CTAs of 256 -> 144 of 448, 90 -> 76 us; 64 rows on 4096,
+// 64 -> 56; head_dim 128, 16 rows x 8 heads on 20000, 58 -> 46.)  A split has min_len
+// keys at least.
+void ac_split(long long units, long long at_once, long long len, long long min_len, long long start, AcParams* p) {
+  double best = 0;
+  p->p_splits = 0;
+  for (int rounds = 1; rounds <= 4; ++rounds) {
+    const long long want = std::max(1ll, std::min(256ll, rounds * at_once / units));
+    const long long keys = std::max(min_len, ((len + want - 1) / want + 63) / 64 * 64), splits = (len + keys - 1) / keys;
+    const double time = (double)((splits * units + at_once - 1) / at_once) * (double)(keys + start);
+    if (p->p_splits && time >= best) continue;
+    best = time;
+    p->p_split_len = (int)keys;
+    p->p_splits = (int)splits;
+  }
 }
 
 template <typename T, int HD>
@@ -1203,15 +1210,15 @@ AcPlan ac_plan(const InfernoAttention* a, AcParams* p) {
   pl.p_tc = ac_prefix_tc(a, pre);
   if (!a->prefix_len) {
   } else if (pl.p_tc) {
-    // one round of CTAs: splits of at least two tiles
+    // starting and joining a CTA takes about as long as eight tiles (13 row tiles x 8
+    // heads on 8000 keys: 101 us in one round of 208 CTAs, 90 in two of 520)
     pl.p_tiles = (int)((pre + ap_rows() - 1) / ap_rows());
-    const long long units = (long long)pl.p_tiles * a->n_kv_heads;
-    const long long want = std::max(1ll, std::min(256ll, (long long)AC_SMS * ap_ctas_per_sm(a->head_dim) / units));
-    const long long sl = ((a->prefix_len + want - 1) / want + 63) / 64 * 64;
-    p->p_split_len = (int)std::max(128ll, sl);
-    p->p_splits = (a->prefix_len + p->p_split_len - 1) / p->p_split_len;
+    ac_split((long long)pl.p_tiles * a->n_kv_heads, (long long)AC_SMS * ap_ctas_per_sm(a->head_dim), a->prefix_len, 128,
+             512, p);
   } else {
-    ac_split((long long)pl.p_tiles * a->n_kv_heads, a->prefix_len, &p->p_splits, &p->p_split_len);
+    // one tile of 16 for each of four key groups at least
+    ac_split((long long)pl.p_tiles * a->n_kv_heads, (long long)AC_SMS * ac_ctas_per_sm(a->type, a->head_dim, pl.p_r),
+             a->prefix_len, 64, 96, p);
   }
   // own part: as many groups of CTAs as fit the GPU at once (two rounds where a
   // group is large, whose remainder would idle), a block of keys each at least.
