@@ -1105,10 +1105,10 @@ struct AcPlan {
 // Rows per CTA for a part with `rows` query rows per KV head and `len` keys.  fp32
 // with few rows goes to ac_vec_kernel in tiles of 4 or 8, where the tensor cores'
 // three products cost more than the lanes' sums: head_dim 256 up to 8 rows (two
-// sequences of 30000: 115 us against 142), or 16 over few keys, which end sooner
-// there (prefix of 500: 11 us against 18; 30000: 178 against 152); 128 up to 4
-// (four of 30000: 74 against 94; 8 rows: 105 against 98); not 64 (4 rows: 69
-// against 58).
+// sequences of 15000 to 30000: 78 us against 107), or 16 over few keys, which end
+// sooner there (prefix of 500: 12.6 us against 14.3; 30000: 97 against 85); 128 up to
+// 4 (four such sequences: 66 against 78; 8 rows: 107 against 79); not 64 (4 rows of
+// 30000: 69 against 58).
 int ac_row_class(int type, int hd, long long rows, int len) {
   if (type == INFERNO_F32 && rows <= (hd == 256 ? (len <= 4096 ? 16 : 8) : hd == 128 ? 4 : 0)) return rows <= 4 ? 4 : 8;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
@@ -1146,18 +1146,21 @@ int ac_ctas_per_sm(int type, int hd, int r) {
   return hd == 64 ? ac_ctas_per_sm<__half, 64>(r) : hd == 128 ? ac_ctas_per_sm<__half, 128>(r) : ac_ctas_per_sm<__half, 256>(r);
 }
 
-// The prefix part of a 16-bit type on tcgen05 or on mma.sync, by the number of
-// products (rows in tiles of 16 x keys x KV heads x head_dim).  tcgen05 streams
-// faster and takes 128 rows at a time, but starts later (TMEM, barriers) and at
-// head_dim 64 waits for its exponentials.  Measured, whole calls, tcgen05 / mma:
-// head_dim 128: 4 rows x 32000 x 8 heads 35 / 41 us, 32 rows 39 / 59; 16 x 16000 x 2
-// 17 / 14; 128 x 500 x 4 12.4 / 13.6; 48 x 300 x 4 12.0 / 11.4; 256: 32 x 8000 x 4 23 /
-// 27, 16 rows 22 / 20; 48 x 300 x 4 14 / 18; 64: 64 x 4000 x 8 17 / 16, 48 x 2000 x 4
-// 12 / 10.
+// The prefix part of a 16-bit type on tcgen05 or on mma.sync.  tcgen05 takes 128 rows
+// at a time, but starts later (TMEM, barriers) and at head_dim 64 waits for its
+// exponentials.  mma.sync with up to 16 rows, its one row tile, streams as fast; above
+// that by the number of products (rows in tiles of 16 x keys x KV heads x head_dim).
+// Whole calls, bf16, tcgen05 / mma.sync, us:
+//   head_dim 64, 4 heads: 32 rows x 16000 15.3 / 13.4 (x 60000, 8 heads 41 / 46), 48 x
+//   4000 10.9 / 10.5, 64 x 4000 11.4 / 12.2, 48 x 16000 15.4 / 18.1
+//   128: 16 x 16000 17.1 / 15.4 (x 60000, 8 heads 49 / 49), 32 x 1000 10.4 / 9.2, 48 x
+//   1000 10.4 / 10.6, 32 x 4000 11.1 / 13.1
+//   256: 16 x 16000 24.5 / 23.6, 48 x 300 12.0 / 15.8, 32 x 1000 13.1 / 13.3, 32 x 4000
+//   15.3 / 21.1
 bool ac_prefix_tc(const InfernoAttention* a, long long rows) {
-  if (a->type == INFERNO_F32) return false;
+  if (a->type == INFERNO_F32 || rows <= 16) return false;
   const double products = (double)((rows + 15) / 16 * 16) * a->prefix_len * a->n_kv_heads * a->head_dim;
-  return products >= (a->head_dim == 64 ? 256e6 : rows > 32 ? 10e6 : 200e6);
+  return products >= (a->head_dim == 64 ? (rows > 32 ? 60e6 : 300e6) : a->head_dim == 128 ? 20e6 : 12e6);
 }
 
 int ac_check(const InfernoAttention* a) {

@@ -226,6 +226,8 @@ ATTN = [
     ("bf16", 17, 8, 8, 1, 64, 1, 9, [9] * 17),
     ("f16", 1, 1, 16, 4, 128, 40001, 5, [5]),                        # four query rows on a long prefix
     ("bf16", 3, 1, 12, 4, 64, 100001, 5, [5, 1, 0]),
+    ("bf16", 17, 1, 4, 4, 128, 9001, 5, [5, 1, 0] * 5 + [2, 2]),     # 17 prefix rows per KV head
+    ("f16", 5, 1, 16, 4, 64, 60001, 70, [70, 64, 1, 65, 0]),
     ("bf16", 65, 1, 16, 4, 64, 4097, 3, [3] * 65),                   # 260 prefix rows, the last four in a tile of their own
 ]
 
