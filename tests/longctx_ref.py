@@ -147,7 +147,7 @@ def attention_ref(q, lens, k, v, pk=None, pv=None, scale=0.0, max_len=None):
                 rel = 2 * (delta + 2.0 ** -22 + s.abs().amax(-1, keepdim=True) * 2.0 ** -22) + (seen + 64) * 2.0 ** -23
                 o, mass = p @ vals[:seen], p @ vals[:seen].abs()
                 out[b, t, h * G:(h + 1) * G] = o
-                # 2^-140: values below the normal range round absolutely
+                # the last term: values below the normal range round absolutely
                 tol[b, t, h * G:(h + 1) * G] = (mass * (rel + (u if dt != torch.float32 else pair)) * 1.01 + o.abs() * u
                                                 + torch.finfo(dt).smallest_normal)
                 gathered[b, h, :seen - P] += p[:, P:].sum(0)
