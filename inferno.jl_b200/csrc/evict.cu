@@ -15,7 +15,7 @@
 // written, so the CTAs of the cluster move K and V in any order.
 //
 // Bound: the bytes of the rows that move (read and written), after a chain of
-// six cluster barriers that few rows cannot hide.
+// up to six cluster barriers that few rows cannot hide.
 #include <algorithm>
 #include <cooperative_groups.h>
 #include "internal.h"
