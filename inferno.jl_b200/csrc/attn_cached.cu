@@ -544,13 +544,21 @@ __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork 
     const uint32_t vt = ring + ((2 * i + 1) % SLOTS) * ITEM;
     // Rows of the call's own tokens, which the tokens before them do not see, may
     // hold anything (padding): 0 times infinity would reach those.  Such rows of V
-    // count as zeros, and the rows of Q that do see them become NaN.
+    // count as zeros, and P is NaN where a row of Q does see one (after the sum: the
+    // weights do not depend on V).
     uint32_t bad = 0;
     if (w.b >= 0 && key0 + AC_KT > w.len - p.n_tok + 1 && p.n_tok > 1) {
       bad = ac_bad_rows<T, ROW>(vt, lane);
-      const uint32_t z_lo = lim_lo <= key0 ? 0u : (1u << min(16, lim_lo - key0)) - 1, z_hi = lim_hi <= key0 ? 0u : (1u << min(16, lim_hi - key0)) - 1;
-      if (bad & z_lo) l_lo = NAN;
-      if (bad & z_hi) l_hi = NAN;
+      if (bad) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int row = 8 * n + 2 * t4 + x;
+            if (bad >> row & 1 && key0 + row < lim_lo) s[n][x] = NAN;
+            if (bad >> row & 1 && key0 + row < lim_hi) s[n][2 + x] = NAN;
+          }
+      }
     }
     if constexpr (!F32) {
       // P rounded to the 16-bit type, as V is: half a step (2^-9, 2^-12) per
@@ -823,7 +831,7 @@ __device__ __forceinline__ void ac_vec_segment(const AcParams& p, const AcWork w
         for (int i = 0; i < D2; ++i) o[r][i].x *= g, o[r][i].y *= g;
       }
     }
-    const float pr = exp2f(x - (m == -INFINITY ? 0.f : m));
+    float pr = exp2f(x - (m == -INFINITY ? 0.f : m));
     l += pr;
     if (w.b >= 0 && p.n_tok > 1 && key0 + KT > w.len - p.n_tok + 1) {
       // rows of the call's own tokens: as in ac_part_kernel
@@ -835,7 +843,7 @@ __device__ __forceinline__ void ac_vec_segment(const AcParams& p, const AcWork w
         if (__any_sync(0xffffffffu, is)) {
 #pragma unroll
           for (int i = 0; i < D2; ++i) vx[k][i] = make_float2(0.f, 0.f);
-          if (my_key == k && key < lim) l = NAN;
+          if (my_key == k && key < lim) pr = NAN;
         }
       }
     }

@@ -1,0 +1,67 @@
+"""Edges of the long-context operators on the GPU: values outside the ordinary
+range.  Plain 64-bit forms and tolerances as in longctx_ref.py."""
+import pytest
+import torch
+
+import longctx_ref as R
+
+pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _case(dtype, B, T, H, kv, d, P, lens, seed=0):
+    """Sequences of lens[b] rows in slices of max(lens), weights gathered."""
+    tid, dt = R.TYPES[dtype]
+    g = _gen(seed)
+    L = max(lens)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(dt)
+
+    c = dict(q=randn(B, T, H, d) * 2, out=torch.full((B, T, H, d), NAN, dtype=dt, device="cuda"))
+    if P:
+        c["pk"], c["pv"] = randn(P, kv, d), randn(P, kv, d)
+    if L:
+        c["k"], c["v"] = randn(B, L, kv, d), randn(B, L, kv, d)
+        c["lens"] = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        c["scores"] = torch.rand(B, kv, L, generator=g, device="cuda")
+    return tid, c
+
+
+def _run(tid, c):
+    """Outputs of a call that leaves the case's own as they are."""
+    c = dict(c, out=c["out"].clone())
+    if "scores" in c:
+        c["scores"] = c["scores"].clone()
+    R.attention(R.attention_args(tid, **c))
+    return c["out"], c.get("scores")
+
+
+# ---------------------------------------------------------------------------
+# weights do not depend on V
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,H,d,T", [("f32", 1, 256, 4), ("f32", 2, 128, 2), ("f32", 3, 64, 5), ("f32", 6, 256, 5),
+                                         ("f32", 20, 128, 2), ("bf16", 2, 128, 3), ("f16", 8, 64, 4),
+                                         ("bf16", 4, 256, 20), ("f32", 1, 256, 1), ("bf16", 2, 128, 1)])
+@pytest.mark.parametrize("value", [INF, NAN])
+@pytest.mark.parametrize("back", [0, 1])
+def test_gathered_weights_do_not_depend_on_v(dtype, H, d, T, value, back):
+    """An infinity or NaN in V of a row of the call's own tokens makes the outputs
+    of the tokens that see it non-finite, and changes no weight and no other output."""
+    if back >= T:
+        pytest.skip("no such token")
+    lens = [90, 33, T]
+    tid, c = _case(dtype, 3, T, 2 * H, 2, d, 40, lens, seed=4)
+    out, scores = _run(tid, c)
+    for b, n in enumerate(lens):
+        c["v"][b, n - 1 - back, 1, d // 3] = value
+    got, got_scores = _run(tid, c)
+    assert torch.equal(got_scores, scores) and scores.isfinite().all()
+    blind = T - 1 - back
+    assert torch.equal(got[:, :blind], out[:, :blind])
+    assert torch.equal(got[:, :, :H], out[:, :, :H])                     # the other KV head
+    assert not got[:, blind:, H:].isfinite().all(-1).any()
