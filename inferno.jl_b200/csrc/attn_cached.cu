@@ -39,14 +39,18 @@ constexpr int AC_KT = 16;                       // keys per tile
 constexpr int AC_SMEM = 227 * 1024, AC_SMEM_HALF = 112 * 1024;
 constexpr int AC_FIN_THREADS = 256;
 
+// P_EXP: P is taken times 2^P_EXP, and so are its sum and O (a part's "largest logit"
+// is that much smaller, so joining parts needs no more).  fp16 has its full precision
+// down to 2^-14 only, and nothing below 2^-25: with the largest weight at 2^15 that is
+// 2^-29 and 2^-40 of it, so that a long tail of small weights is not lost.
 template <typename T>
 struct AcType;
 template <>
-struct AcType<float> { static constexpr bool F32 = true; };
+struct AcType<float> { static constexpr bool F32 = true; static constexpr float P_EXP = 0.f; };
 template <>
-struct AcType<__half> { static constexpr bool F32 = false; };
+struct AcType<__half> { static constexpr bool F32 = false; static constexpr float P_EXP = 15.f; };
 template <>
-struct AcType<__nv_bfloat16> { static constexpr bool F32 = false; };
+struct AcType<__nv_bfloat16> { static constexpr bool F32 = false; static constexpr float P_EXP = 0.f; };
 
 // geometry of one instantiation
 template <typename T, int HD, int R>
@@ -528,7 +532,8 @@ __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork 
 #pragma unroll
       for (int x = 0; x < HD / 8; ++x) o[x][0] *= f_lo, o[x][1] *= f_lo, o[x][2] *= f_hi, o[x][3] *= f_hi;
     }
-    const float z_lo = m_lo == -INFINITY ? 0.f : m_lo, z_hi = m_hi == -INFINITY ? 0.f : m_hi;
+    constexpr float PE = AcType<T>::P_EXP;
+    const float z_lo = m_lo == -INFINITY ? 0.f : m_lo - PE, z_hi = m_hi == -INFINITY ? 0.f : m_hi - PE;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -561,8 +566,9 @@ __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork 
       }
     }
     if constexpr (!F32) {
-      // P rounded to the 16-bit type, as V is: half a step (2^-9, 2^-12) per
-      // term, below the rounding of the output
+      // P rounded to the 16-bit type, as V is: half a step (bf16 2^-8, fp16 2^-11) of
+      // each term at most, as much as the rounding of the output; the sum takes P
+      // unrounded.  A second product for the rest would double those of P V.
       const uint32_t pa[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
                               pack2<T>(s[1][2], s[1][3])};
       // keys 2 t4, 2 t4 + 1 and 8 more of this thread's V values
@@ -622,6 +628,8 @@ __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork 
   }
 
   // ---- merge the key groups ----
+  m_lo -= AcType<T>::P_EXP;
+  m_hi -= AcType<T>::P_EXP;
 #pragma unroll
   for (int of = 1; of <= 2; of <<= 1) {
     l_lo += __shfl_xor_sync(0xffffffffu, l_lo, of);

@@ -8,8 +8,9 @@
 namespace inf {
 
 // Query rows are numbered r = (b * n_tokens + t) * n_heads + h.  A CTA leaves, for
-// each of its rows, one partial result over its keys: the largest logit and the sum
-// and weighted V sum of exp2(logit - largest); logits are in units of log2.
+// each of its rows, one partial result over its keys: the largest logit (less a
+// constant of the kernel and type) and the sum and weighted V sum of exp2(logit -
+// that); logits are in units of log2.
 //
 // The prefix is cut into p_splits equal splits; row r's partial of split s is entry
 // r * p_splits + s.  The own parts are cut evenly whatever lens are: keys are counted

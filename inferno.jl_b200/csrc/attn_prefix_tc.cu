@@ -5,12 +5,13 @@
 // A CTA takes 128 query rows of one KV head against one split of the prefix, in
 // tiles of 64 keys:
 //   S = Q K^T   A = Q tile, B = K tile in shared memory, S in TMEM (two buffers)
-//   P = exp2(scale S - m), rounded to the 16-bit type, back into S's columns
+//   P = exp2(scale S - m), rounded to the 16-bit type (half a step of each weight, as
+//   in attn_cached.cu; the sum takes it unrounded), back into S's columns
 //   O += P V    A = P in TMEM, B = V tile, N-major as it lies in the cache
 // Warps 0-3: softmax, one thread per row (TMEM lane); the running maximum is
-// raised, and O rescaled, only when a row outgrows it by 2^8, since P and the sums
-// hold that much headroom.  Warp 4: K and V tiles by TMA.  Warp 5: issues the MMAs;
-// S of the next tile is issued before P V of this one.  Two CTAs per SM (one at
+// raised, and O rescaled, only when a row outgrows it by 2^8 (fp16 2^4), since P and
+// the sums hold that much headroom.  Warp 4: K and V tiles by TMA.  Warp 5: issues the
+// MMAs; S of the next tile is issued before P V of this one.  Two CTAs per SM (one at
 // head_dim 256) fill each other's gaps.
 //
 // Bound: bytes of K and V up to 128 rows per KV head (a 64-key tile of head_dim 128
@@ -34,7 +35,16 @@ namespace {
 
 constexpr int AP_M = 128, AP_N = 64;
 constexpr int AP_THREADS = 192;
-constexpr float AP_SLACK = 8.0f;    // log2 of what P may exceed 1 by
+
+// SLACK: log2 of what P may exceed the value at the running maximum by, before that is
+// raised.  P_EXP: log2 of P at the running maximum; sum and O are scaled alike, and the
+// part's "largest logit" is that much smaller.  fp16 has its full precision down to
+// 2^-14 only, and nothing below 2^-25: 2^11 at the maximum and 2^15 at most leave it
+// down to 2^-25 (and something down to 2^-36) of the maximum.
+template <typename T>
+struct ApType { static constexpr float SLACK = 8.f, P_EXP = 0.f; };
+template <>
+struct ApType<__half> { static constexpr float SLACK = 4.f, P_EXP = 11.f; };
 
 template <int HD>
 struct ApGeo {
@@ -305,7 +315,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         mx[3] = fmaxf(mx[3], __uint_as_float(u1[i + 1]));
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-      const bool raise = j == 0 || top > m + AP_SLACK;
+      const bool raise = j == 0 || top > m + ApType<T>::SLACK;
       if (j > 0 && __any_sync(0xffffffffu, raise)) {
         // O holds P V up to tile j - 1 once that is done (j - 2 was before S (j) was
         // issued); P V (j) waits for this thread
@@ -329,7 +339,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         tmem_wait_st();
       }
       if (raise) m = top;
-      const float z = m == -INFINITY ? 0.f : m;
+      const float z = m == -INFINITY ? 0.f : m - ApType<T>::P_EXP;
       float sum[2] = {0.f, 0.f};
       uint32_t pk[32];
 #pragma unroll
@@ -388,7 +398,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       if (r < nrows) {
         int tok, h;
         ap_row(p, kvh, r, tok, h);
-        p.part_ml[((long long)tok * p.nh + h) * p.p_splits + split] = make_float2(m, l);
+        p.part_ml[((long long)tok * p.nh + h) * p.p_splits + split] = make_float2(m - ApType<T>::P_EXP, l);
       }
     }
   }

@@ -65,3 +65,40 @@ def test_gathered_weights_do_not_depend_on_v(dtype, H, d, T, value, back):
     assert torch.equal(got[:, :blind], out[:, :blind])
     assert torch.equal(got[:, :, :H], out[:, :, :H])                     # the other KV head
     assert not got[:, blind:, H:].isfinite().all(-1).any()
+
+
+# ---------------------------------------------------------------------------
+# weights far below the largest
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("weight", [4.5e-8, 1e-7, 1e-6, 1e-4])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("B,H,d,P,lens", [
+    (1, 4, 64, 0, [777]), (1, 20, 128, 0, [333]), (1, 40, 256, 0, [100]),      # one, two and four row tiles of own rows
+    (2, 4, 128, 1000, [1, 1]),                                                 # a prefix of few query rows
+    (16, 4, 64, 16001, [1] * 16), (16, 4, 128, 4097, [1] * 16), (16, 4, 256, 3001, [1] * 16),      # and of many
+])
+def test_attention_small_weights_add_up(dtype, weight, B, H, d, P, lens):
+    """Every 16th key takes nearly all the weight and holds V = 0: what is left is
+    the sum over keys of a small weight each.  (P in fp16 keeps its half step down
+    to 2^-14 of what it is scaled to: 2^-25 of the largest at least.)"""
+    tid, c = _case(dtype, B, 1, H, 1, d, P, lens, seed=9)
+    c["q"].zero_()
+    c["q"][..., 0] = 4.0
+    high = torch.log(torch.tensor(1 / weight)).item() / 4.0
+    for k, v in ((c["k"], c["v"]), (c.get("pk"), c.get("pv"))):
+        if k is None:
+            continue
+        k.zero_()
+        v.copy_((torch.rand(v.shape, generator=_gen(3), device="cuda") + 1) * 16384)
+        rows = k.dim() - 3                           # [rows][kv][dim] or [batch][rows][kv][dim]
+        if k.shape[rows] > 1:
+            (k if rows == 0 else k.transpose(0, 1))[::16, ..., 0] = high
+            (v if rows == 0 else v.transpose(0, 1))[::16] = 0
+        else:
+            v.zero_()
+    c.pop("scores")
+    R.attention(R.attention_args(tid, scale=1.0, **c))
+    want, tol, _, _ = R.attention_ref(c["q"], lens, c["k"], c["v"], c.get("pk"), c.get("pv"), 1.0)
+    assert (want > 100 * torch.finfo(c["out"].dtype).smallest_normal).all()
+    err = (c["out"].double() - want).abs()
+    assert (err <= tol).all(), f"worst error / tolerance {float((err / tol).max())}"
