@@ -245,8 +245,12 @@ int inferno_rope(const InfernoRope* r, void* stream);
  * Query head h reads KV head h / (n_heads / n_kv_heads); no RoPE, norm or gate
  * is applied.  A token that sees no row gets zeros.  lens are clamped to
  * [0, max_len].  Rows that a token does not see do not reach its output,
- * whatever they hold (rows from lens[b] on, and those of the tokens behind it);
- * non-finite values in rows that it sees make its output non-finite.
+ * whatever they hold (rows from lens[b] on, and those of the tokens behind it).
+ * In rows that it sees, a logit of -inf has weight 0 (with no other kind the
+ * token gets zeros), one of +inf or NaN makes its output and the weights that
+ * it gathers NaN, and an infinity or NaN in V makes its output non-finite,
+ * whatever the weight.  (fp32 values of V from 2^128 (1 - 2^-12) on may count
+ * as infinite.)
  * scores (optional, fp32): scores[(b * n_kv_heads + h) * score_stride + j]
  * gains the weight that own row j got, summed over the tokens and query heads
  * of KV head h; entries from lens[b] on are left as they are.

@@ -306,6 +306,39 @@ __device__ __forceinline__ long long ac_entry(const AcParams& p, const AcWork& w
   return ((long long)(b * p.n_tok + t) * p.nh + h) * p.p_splits + w.split;
 }
 
+// fp32: the logits of rows r and r + 8 of a part with keys 2 t4, 2 t4 + 1 and 8 more of
+// the tile at kt, in the accumulator layout, in place of those of s that are NaN
+template <int HD>
+__device__ __forceinline__ void ac_plain_logits(const AcParams& p, const AcWork& w, int r, uint32_t kt, int t4, float (&s)[2][4]) {
+  const float* q[2] = {nullptr, nullptr};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (r + 8 * i < w.nrows) {
+      int b, t, h;
+      ac_row(p, w, r + 8 * i, b, t, h);
+      q[i] = (const float*)p.q + (long long)(b * p.n_tok + t) * p.q_stride + (long long)h * HD;
+    }
+  float e[2][4] = {};
+#pragma unroll 1
+  for (int c = 0; c < HD / 4; ++c) {
+    float4 x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = q[i] ? *(const float4*)(q[i] + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 k = lds_f4(tile_addr<HD * 4>(kt, 8 * n + 2 * t4 + j, c));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          e[n][2 * i + j] = fmaf(x[i].w, k.w, fmaf(x[i].z, k.z, fmaf(x[i].y, k.y, fmaf(x[i].x, k.x, e[n][2 * i + j]))));
+      }
+  }
+#pragma unroll
+  for (int a = 0; a < 8; ++a)
+    if (s[a >> 2][a & 3] != s[a >> 2][a & 3]) s[a >> 2][a & 3] = e[a >> 2][a & 3];
+}
+
 // one piece of work of a CTA, from its first copies to its partial results
 template <typename T, int HD, int R>
 __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork w, uint8_t* smem) {
@@ -497,6 +530,12 @@ __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork 
       }
 #pragma unroll
       for (int a = 0; a < 8; ++a) s[a >> 2][a & 3] += hl[a >> 2][a & 3] + lh[a >> 2][a & 3];
+      // An infinity in Q or K has the rest inf - inf, and so NaN for the logit that
+      // may be -inf: such logits are formed again from the values themselves.
+      bool odd = false;
+#pragma unroll
+      for (int a = 0; a < 8; ++a) odd |= s[a >> 2][a & 3] != s[a >> 2][a & 3];
+      if (__any_sync(0xffffffffu, odd)) ac_plain_logits<HD>(p, w, r_lo, kt, t4, s);
     }
     // ---- running softmax ----
     float mx_lo = -INFINITY, mx_hi = -INFINITY;

@@ -68,6 +68,71 @@ def test_gathered_weights_do_not_depend_on_v(dtype, H, d, T, value, back):
 
 
 # ---------------------------------------------------------------------------
+# infinite logits
+# ---------------------------------------------------------------------------
+INFINITE = [
+    # type, batch, heads, kv, dim, prefix, lens
+    ("f32", 1, 8, 2, 256, 0, [70]),                # CUDA cores, four rows
+    ("f32", 3, 8, 2, 256, 300, [70, 1, 5]),        # eight and sixteen rows
+    ("f32", 2, 4, 2, 128, 33, [9, 200]),
+    ("f32", 1, 32, 2, 128, 0, [70]),               # tensor cores, one row tile
+    ("f32", 2, 24, 1, 64, 200, [70, 64]),          # two, and four
+    ("f32", 2, 17, 1, 256, 50, [33, 16]),
+    ("bf16", 2, 8, 2, 128, 50, [70, 1]),
+    ("f16", 2, 8, 2, 64, 50, [70, 33]),
+    ("bf16", 24, 8, 2, 128, 3000, [1 + b for b in range(24)]),      # tcgen05
+    ("f16", 24, 8, 2, 64, 6000, [40] * 24),
+    ("bf16", 24, 8, 2, 256, 3000, [40] * 24),
+]
+
+
+@pytest.mark.parametrize("dtype,B,H,kv,d,P,lens", INFINITE)
+def test_a_logit_of_minus_infinity_has_no_weight(dtype, B, H, kv, d, P, lens):
+    """Whichever kernel takes the call: as if the row were not there."""
+    tid, c = _case(dtype, B, 1, H, kv, d, P, lens, seed=7)
+    c["q"][..., 0] = c["q"][..., 0].abs() + 0.5
+    for b, n in enumerate(lens):
+        c["k"][b, n - 1, :, 0] = -INF
+    if P:
+        c["pk"][0, :, 0] = -INF
+    out, scores = _run(tid, c)
+    less = [n - 1 for n in lens]
+    want, tol, gathered, gtol = R.attention_ref(c["q"], less, c["k"], c["v"], c["pk"][1:] if P else None,
+                                                c["pv"][1:] if P else None)
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), f"worst error / tolerance {float((err / tol).max())}"
+    got = scores.double() - c["scores"].double()
+    assert ((got - gathered).abs() <= gtol + scores.double() * 2.0 ** -24).all()
+    for b, n in enumerate(lens):
+        assert torch.equal(scores[b, :, n - 1:], c["scores"][b, :, n - 1:])
+
+
+@pytest.mark.parametrize("dtype,B,H,kv,d,P,lens", INFINITE)
+def test_logits_of_minus_infinity_alone_give_zeros(dtype, B, H, kv, d, P, lens):
+    tid, c = _case(dtype, B, 1, H, kv, d, P, lens, seed=6)
+    c["q"][..., 0] = c["q"][..., 0].abs() + 0.5
+    c["k"][..., 0] = -INF
+    if P:
+        c["pk"][..., 0] = -INF
+    out, scores = _run(tid, c)
+    assert (out == 0).all() and torch.equal(scores, c["scores"])
+
+
+@pytest.mark.parametrize("dtype,B,H,kv,d,P,lens", INFINITE)
+def test_a_logit_of_infinity_spoils_its_row(dtype, B, H, kv, d, P, lens):
+    """NaN for the heads that see it, the same bits for the others."""
+    tid, c = _case(dtype, B, 1, H, kv, d, P, lens, seed=8)
+    c["q"][..., 0] = c["q"][..., 0].abs() + 0.5
+    out, scores = _run(tid, c)
+    c["k"][0, lens[0] // 2, 0, 0] = INF
+    got, got_scores = _run(tid, c)
+    G = H // kv
+    assert got[0, 0, :G].isnan().all() and got_scores[0, 0, :lens[0]].isnan().all()
+    assert torch.equal(got[1:], out[1:]) and torch.equal(got[0, 0, G:], out[0, 0, G:])
+    assert torch.equal(got_scores[1:], scores[1:]) and torch.equal(got_scores[0, 1:], scores[0, 1:])
+
+
+# ---------------------------------------------------------------------------
 # weights far below the largest
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("weight", [4.5e-8, 1e-7, 1e-6, 1e-4])
