@@ -257,7 +257,10 @@ int inferno_rope(const InfernoRope* r, void* stream);
  * q and out [batch * n_tokens][n_heads][head_dim] with q_stride / out_stride
  * elements between token rows; out may be q, and overlaps nothing else.
  * head_dim 64, 128 or 256; pointers and strides multiples of 16 bytes (lens and
- * scores: of 4).  Results do not depend on timing (no atomics). */
+ * scores: of 4).  Results do not depend on timing (no atomics).
+ * The kernel for many query rows on a 16-bit prefix waits for its own copies and
+ * products; should such a wait run out, the outputs concerned (and the weights
+ * that they gather) are NaN and inferno_device_error reports it. */
 typedef struct InfernoAttention {
   int32_t struct_size;
   int32_t type;
@@ -277,6 +280,10 @@ typedef struct InfernoAttention {
  * buffer), or a negative status; reads no pointer but whether scores is set */
 int64_t inferno_attention_cached_workspace(const InfernoAttention* a);
 int inferno_attention_cached(const InfernoAttention* a, void* workspace, int64_t workspace_bytes, void* stream);
+/* Failure-path check (debug / tests): the same call with every such wait running
+ * out at once; refused where the call has none.  Expected result: status 0, NaN
+ * outputs, inferno_device_error 1, the context still usable. */
+int inferno_debug_attention_timeout(const InfernoAttention* a, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Eviction: cuts each (sequence, KV head) with lens[b] > budget to budget
  * rows.  Kept are, in this order: rows whose position slot_pos is < n_sink or

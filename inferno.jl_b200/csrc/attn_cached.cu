@@ -1400,8 +1400,9 @@ extern "C" int64_t inferno_attention_cached_workspace(const InfernoAttention* a)
   return (int64_t)ac_plan(a, &p).bytes;
 }
 
-extern "C" int inferno_attention_cached(const InfernoAttention* a, void* workspace, int64_t workspace_bytes,
-                                        void* stream) {
+namespace {
+
+int ac_call(const InfernoAttention* a, void* workspace, int64_t workspace_bytes, void* stream, bool give_up) {
   int rc = ac_check(a);
   if (rc) return rc;
   if (a->batch == 0) return 0;
@@ -1429,6 +1430,8 @@ extern "C" int inferno_attention_cached(const InfernoAttention* a, void* workspa
     return set_error(INFERNO_EINVAL, "attention_cached: lens or scores is not a multiple of 4 bytes");
   AcParams p{};
   const AcPlan pl = ac_plan(a, &p);
+  if (give_up && !(pl.p_tc && p.p_splits))
+    return set_error(INFERNO_EINVAL, "attention_cached: no bounded waits in a call of these sizes");
   if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (int64_t)pl.bytes)
     return set_error(INFERNO_EINVAL, "attention_cached: workspace of %lld bytes, %lld needed (256-byte aligned)",
                      (long long)workspace_bytes, (long long)pl.bytes);
@@ -1451,9 +1454,21 @@ extern "C" int inferno_attention_cached(const InfernoAttention* a, void* workspa
   p.head = (int*)((char*)workspace + pl.off_head);
   p.logits = (float*)((char*)workspace + pl.off_logits);
   cudaStream_t st = (cudaStream_t)stream;
-  if (pl.p_tc && p.p_splits && (rc = launch_attn_prefix_tc(a->type, a->head_dim, p, pl.p_tiles, st))) return rc;
+  if (pl.p_tc && p.p_splits && (rc = launch_attn_prefix_tc(a->type, a->head_dim, p, pl.p_tiles, give_up, st))) return rc;
   const cudaError_t e = a->type == INFERNO_F32   ? ac_run_hd<float>(a->head_dim, p, pl, st)
                         : a->type == INFERNO_F16 ? ac_run_hd<__half>(a->head_dim, p, pl, st)
                                                  : ac_run_hd<__nv_bfloat16>(a->head_dim, p, pl, st);
   return e == cudaSuccess ? 0 : set_error(INFERNO_ECUDA, "attention_cached launch: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" int inferno_attention_cached(const InfernoAttention* a, void* workspace, int64_t workspace_bytes,
+                                        void* stream) {
+  return ac_call(a, workspace, workspace_bytes, stream, false);
+}
+
+extern "C" int inferno_debug_attention_timeout(const InfernoAttention* a, void* workspace, int64_t workspace_bytes,
+                                               void* stream) {
+  return ac_call(a, workspace, workspace_bytes, stream, true);
 }

@@ -58,6 +58,7 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 // the prefix part on tcgen05 (attn_prefix_tc.cu): query rows per CTA, CTAs per SM
 int ap_rows();
 int ap_ctas_per_sm(int hd);
-int launch_attn_prefix_tc(int type, int hd, const AcParams& p, int row_tiles, cudaStream_t st);
+// give_up: every wait that the work depends on runs out at once (a test of that path)
+int launch_attn_prefix_tc(int type, int hd, const AcParams& p, int row_tiles, bool give_up, cudaStream_t st);
 
 }  // namespace inf

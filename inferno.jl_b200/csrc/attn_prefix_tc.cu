@@ -57,9 +57,12 @@ struct ApGeo {
   static constexpr int CTAS = HD == 256 ? 1 : 2;
 };
 
-// A poll sleeps for up to about 4 us, so this gives up after about two seconds.
-__device__ __forceinline__ bool ap_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t i = 0; i < (1u << 19); ++i)
+// A poll sleeps for up to about 4 us, so AP_POLLS give up after about two seconds.
+// A CTA that gives up still waits for its own copies and MMAs in flight, and leaves
+// NaN as the sums of its rows, so that what they join does not look like a result.
+constexpr uint32_t AP_POLLS = 1u << 19;
+__device__ __forceinline__ bool ap_wait(uint64_t* bar, uint32_t parity, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   atomicExch(&ap_error, DERR_MBAR_TIMEOUT);
   return false;
@@ -129,7 +132,7 @@ struct alignas(64) ApMaps {
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const __grid_constant__ AcParams p, const __grid_constant__ ApMaps maps, int row_tiles) {
+__global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const __grid_constant__ AcParams p, const __grid_constant__ ApMaps maps, int row_tiles, uint32_t polls) {
   using G = ApGeo<HD>;
   constexpr int ST = G::STAGES;
   extern __shared__ uint8_t ap_smem[];
@@ -148,7 +151,8 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
   uint64_t* p_full = s_full + 2;          // 2
   uint64_t* pv_done = p_full + 2;         // 1: phase j is P V of tile j
   uint64_t* o_done = pv_done + 1;         // 1: all of them
-  uint64_t* q_full = o_done + 1;          // 1
+  uint64_t* drained = o_done + 1;         // 1: those issued before a wait ran out
+  uint64_t* q_full = drained + 1;         // 1
   uint32_t* s_tmem = (uint32_t*)(q_full + 1);
 
   int x = blockIdx.x;
@@ -172,6 +176,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
     }
     mbar_init(pv_done, 1);
     mbar_init(o_done, 1);
+    mbar_init(drained, 1);
     mbar_init(q_full, AP_M);
     fence_mbar_init();
   }
@@ -188,28 +193,25 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
   if (warp == 4) {
     // ================= K / V producer =================
     if (lane == 0) {
-      int issued = 0;
+      int k_issued = 0, v_issued = 0;
       for (int j = 0; j < tiles; ++j) {
         const int st = j % ST, key = j0 + j * AP_N;
-        if (j >= ST && !ap_wait(&k_empty[st], ((j / ST) - 1) & 1)) break;
+        if (j >= ST && !ap_wait(&k_empty[st], ((j / ST) - 1) & 1, polls)) break;
         mbar_arrive_expect_tx(&k_full[st], G::TILE);
 #pragma unroll
         for (int s = 0; s < G::SUB; ++s)
           tma_load_2d(s_k + st * G::TILE + s * AP_N * 128, &maps.k, kvh * HD + s * 64, key, &k_full[st]);
-        if (j >= ST && !ap_wait(&v_empty[st], ((j / ST) - 1) & 1)) {
-          ap_wait(&k_full[st], (j / ST) & 1);           // its own copies land before the CTA leaves
-          break;
-        }
+        k_issued = j + 1;
+        if (j >= ST && !ap_wait(&v_empty[st], ((j / ST) - 1) & 1, polls)) break;
         mbar_arrive_expect_tx(&v_full[st], G::TILE);
 #pragma unroll
         for (int s = 0; s < G::SUB; ++s)
           tma_load_2d(s_v + st * G::TILE + s * AP_N * 128, &maps.v, kvh * HD + s * 64, key, &v_full[st]);
-        issued = j + 1;
+        v_issued = j + 1;
       }
-      for (int j = max(0, issued - ST); j < issued; ++j) {
-        ap_wait(&k_full[j % ST], (j / ST) & 1);
-        ap_wait(&v_full[j % ST], (j / ST) & 1);
-      }
+      // its own copies land before the CTA leaves: the last one of each stage
+      for (int j = max(0, k_issued - ST); j < k_issued; ++j) ap_wait(&k_full[j % ST], (j / ST) & 1, AP_POLLS);
+      for (int j = max(0, v_issued - ST); j < v_issued; ++j) ap_wait(&v_full[j % ST], (j / ST) & 1, AP_POLLS);
     }
     __syncwarp();
   } else if (warp == 5) {
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         umma_commit(&s_full[j & 1]);
         umma_commit(&k_empty[j % ST]);
       };
-      bool ok = ap_wait(q_full, 0) && ap_wait(&k_full[0], 0);
+      bool ok = ap_wait(q_full, 0, polls) && ap_wait(&k_full[0], 0, polls);
       if (ok) {
         tc_fence_after();
         issue_s(0);
@@ -237,12 +239,12 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       for (int j = 0; j < tiles && ok; ++j) {
         if (j + 1 < tiles) {
           // S(j + 1) takes the columns of P(j - 1), which P V (j - 1) reads
-          ok = (j == 0 || ap_wait(pv_done, (j - 1) & 1)) && ap_wait(&k_full[(j + 1) % ST], ((j + 1) / ST) & 1);
+          ok = (j == 0 || ap_wait(pv_done, (j - 1) & 1, polls)) && ap_wait(&k_full[(j + 1) % ST], ((j + 1) / ST) & 1, polls);
           if (!ok) break;
           tc_fence_after();
           issue_s(j + 1);
         }
-        ok = ap_wait(&p_full[j & 1], (j >> 1) & 1) && ap_wait(&v_full[j % ST], (j / ST) & 1);
+        ok = ap_wait(&p_full[j & 1], (j >> 1) & 1, polls) && ap_wait(&v_full[j % ST], (j / ST) & 1, polls);
         if (!ok) break;
         tc_fence_after();
         const uint32_t vb = smem_u32(s_v + (j % ST) * G::TILE);
@@ -253,8 +255,8 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         umma_commit(pv_done);
         umma_commit(&v_empty[j % ST]);
       }
-      umma_commit(o_done);
-      if (!ok) ap_wait(o_done, 0);          // no MMA in flight when TMEM is freed
+      umma_commit(ok ? o_done : drained);
+      if (!ok) ap_wait(drained, 0, AP_POLLS);     // no MMA in flight when TMEM is freed
     }
     __syncwarp();
   } else {
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
-      ok = ap_wait(&s_full[j & 1], (j >> 1) & 1);
+      ok = ap_wait(&s_full[j & 1], (j >> 1) & 1, polls);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       if (j > 0 && __any_sync(0xffffffffu, raise)) {
         // O holds P V up to tile j - 1 once that is done (j - 2 was before S (j) was
         // issued); P V (j) waits for this thread
-        ok = ap_wait(pv_done, (j - 1) & 1);
+        ok = ap_wait(pv_done, (j - 1) & 1, polls);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
     // ---- partial result ----
     // its own barrier: pv_done may be one or two phases on by now, and a parity
     // tells a phase only from its neighbours
-    ok = ok && ap_wait(o_done, 0);
+    ok = ok && ap_wait(o_done, 0, polls);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       // O leaves by whole 128-byte lines: 32 columns of a warp's 32 rows turn through
@@ -400,6 +402,10 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         ap_row(p, kvh, r, tok, h);
         p.part_ml[((long long)tok * p.nh + h) * p.p_splits + split] = make_float2(m - ApType<T>::P_EXP, l);
       }
+    } else if (row0 + tid < nrows) {
+      int tok, h;
+      ap_row(p, kvh, row0 + tid, tok, h);
+      p.part_ml[((long long)tok * p.nh + h) * p.p_splits + split] = make_float2(0.f, NAN);
     }
   }
   tc_fence_before();
@@ -445,7 +451,7 @@ int ap_map(CUtensorMap* m, int type, const void* base, long long width, int rows
 }
 
 template <typename T, int HD>
-cudaError_t ap_launch(const AcParams& p, const ApMaps& maps, int row_tiles, cudaStream_t st) {
+cudaError_t ap_launch(const AcParams& p, const ApMaps& maps, int row_tiles, uint32_t polls, cudaStream_t st) {
   using G = ApGeo<HD>;
   static DeviceOnce once;
   const cudaError_t e = once.run([] {
@@ -454,14 +460,14 @@ cudaError_t ap_launch(const AcParams& p, const ApMaps& maps, int row_tiles, cuda
   if (e != cudaSuccess) return e;
   const long long blocks = (long long)row_tiles * p.nkv * p.p_splits;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  ap_kernel<T, HD><<<(unsigned)blocks, AP_THREADS, G::SMEM, st>>>(p, maps, row_tiles);
+  ap_kernel<T, HD><<<(unsigned)blocks, AP_THREADS, G::SMEM, st>>>(p, maps, row_tiles, polls);
   return cudaGetLastError();
 }
 template <typename T>
-cudaError_t ap_launch_hd(int hd, const AcParams& p, const ApMaps& maps, int row_tiles, cudaStream_t st) {
-  return hd == 64    ? ap_launch<T, 64>(p, maps, row_tiles, st)
-         : hd == 128 ? ap_launch<T, 128>(p, maps, row_tiles, st)
-                     : ap_launch<T, 256>(p, maps, row_tiles, st);
+cudaError_t ap_launch_hd(int hd, const AcParams& p, const ApMaps& maps, int row_tiles, uint32_t polls, cudaStream_t st) {
+  return hd == 64    ? ap_launch<T, 64>(p, maps, row_tiles, polls, st)
+         : hd == 128 ? ap_launch<T, 128>(p, maps, row_tiles, polls, st)
+                     : ap_launch<T, 256>(p, maps, row_tiles, polls, st);
 }
 
 }  // namespace
@@ -469,14 +475,15 @@ cudaError_t ap_launch_hd(int hd, const AcParams& p, const ApMaps& maps, int row_
 int ap_rows() { return AP_M; }
 int ap_ctas_per_sm(int hd) { return hd == 256 ? ApGeo<256>::CTAS : ApGeo<128>::CTAS; }
 
-int launch_attn_prefix_tc(int type, int hd, const AcParams& p, int row_tiles, cudaStream_t st) {
+int launch_attn_prefix_tc(int type, int hd, const AcParams& p, int row_tiles, bool give_up, cudaStream_t st) {
   ApMaps maps;
   const long long width = (long long)p.nkv * hd;
   int rc = ap_map(&maps.k, type, p.pk, width, p.prefix_len);
   if (!rc) rc = ap_map(&maps.v, type, p.pv, width, p.prefix_len);
   if (rc) return rc;
-  const cudaError_t e = type == INFERNO_F16 ? ap_launch_hd<__half>(hd, p, maps, row_tiles, st)
-                                            : ap_launch_hd<__nv_bfloat16>(hd, p, maps, row_tiles, st);
+  const uint32_t polls = give_up ? 0 : AP_POLLS;
+  const cudaError_t e = type == INFERNO_F16 ? ap_launch_hd<__half>(hd, p, maps, row_tiles, polls, st)
+                                            : ap_launch_hd<__nv_bfloat16>(hd, p, maps, row_tiles, polls, st);
   return e == cudaSuccess ? 0 : set_error(INFERNO_ECUDA, "attention_cached launch: %s", cudaGetErrorString(e));
 }
 

@@ -82,7 +82,7 @@ EXPORTS = [
     "inferno_gguf_data_offset", "inferno_gguf_key", "inferno_gguf_tensor_info", "inferno_gguf_get_int",
     "inferno_gguf_get_float", "inferno_gguf_get_string", "inferno_gguf_get_array", "inferno_engine_load_gguf",
     "inferno_rope", "inferno_attention_cached_workspace", "inferno_attention_cached", "inferno_cache_evict_workspace",
-    "inferno_cache_evict",
+    "inferno_cache_evict", "inferno_debug_attention_timeout",
 ]
 
 _lib = None
@@ -163,6 +163,7 @@ def _sig(L0):
         getattr(L, nm).argtypes = [p, p, i64, p]
         getattr(L, nm + "_workspace").argtypes = [p]
         getattr(L, nm + "_workspace").restype = i64
+    L.inferno_debug_attention_timeout.argtypes = [p, p, i64, p]
     L.inferno_attention_step.argtypes = [p, p, p, p, p, f, i, i, i, i, f, p, p, i, i, i, p, p]
 
 

@@ -1,9 +1,12 @@
 """Edges of the long-context operators on the GPU: values outside the ordinary
-range.  Plain 64-bit forms and tolerances as in longctx_ref.py."""
+range, and waits that run out.  Plain 64-bit forms and tolerances as in longctx_ref.py."""
+import ctypes as C
+
 import pytest
 import torch
 
 import longctx_ref as R
+from inferno_b200._lib import call, lib
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -167,3 +170,28 @@ def test_attention_small_weights_add_up(dtype, weight, B, H, d, P, lens):
     assert (want > 100 * torch.finfo(c["out"].dtype).smallest_normal).all()
     err = (c["out"].double() - want).abs()
     assert (err <= tol).all(), f"worst error / tolerance {float((err / tol).max())}"
+
+
+# ---------------------------------------------------------------------------
+# waits that run out
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,B,H,kv,d,P", [("bf16", 24, 8, 2, 128, 3000), ("f16", 24, 8, 2, 64, 6000),
+                                              ("bf16", 40, 8, 2, 256, 3000)])
+def test_a_wait_that_runs_out_gives_nan(dtype, B, H, kv, d, P):
+    """Whatever an earlier call left in the workspace: NaN outputs and weights, the
+    device error word set, and the next call as ever."""
+    tid, c = _case(dtype, B, 1, H, kv, d, P, [40] * B, seed=5)
+    a = R.attention_args(tid, **c)
+    ws = R.attention_workspace(a)
+    before = c["scores"].clone()
+    R.attention(a, ws)
+    want, want_scores = c["out"].clone(), c["scores"].clone()
+    c["scores"].copy_(before)
+    assert lib().inferno_device_error(0, 1) == 0
+    call("inferno_debug_attention_timeout", C.byref(a), C.c_void_p(ws.data_ptr()), ws.numel(), R.stream())
+    assert c["out"].isnan().all() and c["scores"].isnan().all()
+    assert lib().inferno_device_error(0, 1) == 1
+    c["scores"].copy_(before)
+    R.attention(a, ws)
+    assert torch.equal(c["out"], want) and torch.equal(c["scores"], want_scores)
+    assert lib().inferno_device_error(0, 0) == 0
