@@ -203,7 +203,8 @@ int inferno_gdn_chunked(int T, int n_heads, int dk, int dv, const float* q, cons
  *     ceil(d(beta_slow)), d(n) = rope_dim log(orig_ctx / (2 pi n)) / (2 log theta)
  *     (the ends held within [0, rope_dim - 1]); cos and sin are multiplied by
  *     mscale.
- * Angles are reduced in double, so positions up to 2^31 - 1 keep fp32 accuracy.
+ * Whole turns are dropped exactly, so angles keep fp32 accuracy (2e-7) up to
+ * position 2^31 - 1.
  * In place (x_out == x with equal strides) is allowed; any other overlap of an
  * output row with an input or output row is refused.  Rows may have any
  * alignment of the element type (16-byte aligned ones are faster). */

@@ -10,10 +10,12 @@
 // instructions: 96 us for 16383 tokens x 40 heads of 128 bf16, and more items in
 // flight only made it slower.)
 //
-// Angles: f_i / (2 pi) is a double, so positions[t] * f_i / (2 pi) has the turn
-// exact to 2^-52 of itself; the whole turns are dropped in double and the rest,
-// at most half a turn, goes to sincospi in fp32.  The error is that of an fp32
-// angle below pi (about 1e-7) at any position.
+// Angles: f_i / (2 pi) is a double and a rest, 2^-54 of itself off at most (see the
+// host), and its product with the position is taken exactly, the double's and the
+// rest's; the whole turns are dropped in double and what is left, at most half a
+// turn, goes to sincospi in fp32.  Up to 2^28.4 turns (position 2^31 - 1) the angle
+// is off by 2 pi (2^-26 + 2^-26), 2e-7, from the frequency and from its rounding to
+// fp32; by half of that up to position 2^28.
 //
 // Bound: bytes, each value read and written once.
 #include <algorithm>
@@ -47,6 +49,7 @@ struct RopeParams {
   FastDiv by_units, by_v;
   float gain, sign;                      // factor of cos and sin; -1: rotate back
   double turns[ROPE_MAX_PAIRS];          // f_i / (2 pi), without freq_factors
+  float turns_rest[ROPE_MAX_PAIRS];      // what the double leaves of it
 };
 
 template <typename T, int V>
@@ -111,10 +114,16 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_kernel(const __grid_cons
   const int t0 = blockIdx.x * p.tb, nt = min(p.tb, p.n_tokens - t0);
   for (int i = threadIdx.x; i < nt * half; i += ROPE_THREADS) {
     const int t = i / half, c = i - t * half;
-    double turn = p.turns[c];
-    if (p.freq_factors) turn /= (double)__ldg(p.freq_factors + c);
-    turn *= (double)__ldg(p.positions + t0 + t);
-    turn -= rint(turn);
+    double f = p.turns[c], rest = p.turns_rest[c];
+    if (p.freq_factors) {
+      const double w = __ldg(p.freq_factors + c), g = f / w;
+      rest = (fma(-g, w, f) + rest) / w;
+      f = g;
+    }
+    const double at = __ldg(p.positions + t0 + t);
+    double turn = f * at;
+    rest = fma(f, at, -turn) + rest * at;
+    turn = turn - rint(turn) + rest;
     float sn, cn;
     sincospif(2.0f * (float)turn, &sn, &cn);
     cs[i] = make_float2(cn * p.gain, sn * p.gain * p.sign);
@@ -359,9 +368,16 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
   p.gain = r->mscale != 0.0f ? r->mscale
            : r->scaling == INFERNO_ROPE_SCALE_PARTS && r->factor > 1.0f ? (float)(0.1 * std::log((double)r->factor) + 1.0)
                                                                         : 1.0f;
-  // f_i by repeated multiplication: 256 steps lose at most 2^-44 of f_i
+  // f_i by repeated multiplication in extended precision (64 bits): the ratio is off by
+  // 2^-63 of itself and each product by 2^-64, so 255 steps lose 2^-54 of f_i.  (In
+  // double they lost 1e-6 in the angle at far positions, or 2e-5 with theta 1.5, whose
+  // later pairs turn nearly as fast as the first.)  The ratio is pow's in double after
+  // one Newton step for theta ratio^half = 1: powl takes 400 ns of a call of 4 us.
   const double two_pi = 6.283185307179586476925286766559;
-  const double ratio = std::pow((double)r->theta, -2.0 / r->rope_dim);
+  long double ratio = std::pow((double)r->theta, -2.0 / r->rope_dim), power = r->theta, square = ratio;
+  for (int n = half; n; n >>= 1, square *= square)
+    if (n & 1) power *= square;
+  ratio -= ratio * (power - 1.0L) / half;
   double low = 0, high = 0;
   if (r->scaling == INFERNO_ROPE_SCALE_PARTS) {
     auto dim = [&](double turns) {
@@ -370,15 +386,16 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
     low = std::max(std::floor(dim(fast)), 0.0);
     high = std::min(std::ceil(dim(slow)), r->rope_dim - 1.0);
   }
-  double f = 1.0 / two_pi;
+  long double f = 1.0L / 6.283185307179586476925286766559005768L;
   for (int i = 0; i < half; ++i, f *= ratio) {
-    double g = f;
+    long double g = f;
     if (r->scaling == INFERNO_ROPE_SCALE_LINEAR) g = f / r->factor;
     if (r->scaling == INFERNO_ROPE_SCALE_PARTS) {
-      const double ramp = std::min(std::max((i - low) / std::max(high - low, 0.001), 0.0), 1.0);
-      g = f * (1.0 - ramp) + f / r->factor * ramp;
+      const long double ramp = std::min(std::max((i - low) / std::max(high - low, 0.001), 0.0), 1.0);
+      g = f * (1.0L - ramp) + f / r->factor * ramp;
     }
-    p.turns[i] = g;
+    p.turns[i] = (double)g;
+    p.turns_rest[i] = (float)(g - (long double)p.turns[i]);
   }
 
   // tokens per block: about four units for every team, fewer when there are too

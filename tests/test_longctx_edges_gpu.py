@@ -1,6 +1,7 @@
 """Edges of the long-context operators on the GPU: values outside the ordinary
 range, and waits that run out.  Plain 64-bit forms and tolerances as in longctx_ref.py."""
 import ctypes as C
+import decimal
 
 import pytest
 import torch
@@ -169,6 +170,50 @@ def test_attention_small_weights_add_up(dtype, weight, B, H, d, P, lens):
     want, tol, _, _ = R.attention_ref(c["q"], lens, c["k"], c["v"], c.get("pk"), c.get("pv"), 1.0)
     assert (want > 100 * torch.finfo(c["out"].dtype).smallest_normal).all()
     err = (c["out"].double() - want).abs()
+    assert (err <= tol).all(), f"worst error / tolerance {float((err / tol).max())}"
+
+
+# ---------------------------------------------------------------------------
+# far positions
+# ---------------------------------------------------------------------------
+def _far_angles(positions, rope_dim, theta, factors=None):
+    """Angles within [-pi, pi] from 60 decimal digits."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        two_pi = 2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+        log = decimal.Decimal(theta).ln()
+        rows = []
+        for at in positions:
+            row = []
+            for i in range(rope_dim // 2):
+                a = at * (-log * 2 * i / rope_dim).exp()
+                if factors is not None:
+                    a /= decimal.Decimal(factors[i])
+                row.append(float(a - (a / two_pi).to_integral_value() * two_pi))
+            rows.append(row)
+    return torch.tensor(rows, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("theta,r,with_factors", [(1e4, 512, False), (1.5, 512, False), (2.0, 64, True), (5e5, 128, True)])
+def test_rope_far_positions(theta, r, with_factors, layout):
+    """fp32 up to position 2^31 - 1.  The turn is exact to 2^-26 from its rounding
+    to fp32 and 2^-26 from the frequency (2^-54 of itself, 2^28.4 turns at most): 2 pi
+    2^-25 in the angle, which moves a value by at most |a| + |b| of it; sincospi is
+    off by 2 ulp (2^-23); two products and a sum round (3 * 2^-24)."""
+    n, H = 3, 2
+    positions = [(1 << 31) - 1, 1234567891, 3]
+    g = _gen(11)
+    x = torch.randn(n, H * r, generator=g, device="cuda")
+    pos = torch.tensor(positions, dtype=torch.int32, device="cuda")
+    ff = torch.rand(r // 2, generator=g, device="cuda") + 0.75 if with_factors else None
+    y = torch.empty_like(x)
+    R.rope(R.rope_args(0, x, None, None, y, n_tokens=n, n_heads=H, n_kv_heads=0, head_dim=r, rope_dim=r, positions=pos,
+                       layout=layout, theta=theta, freq_factors=R.ptr(ff)))
+    ang = _far_angles(positions, r, theta, ff.tolist() if with_factors else None)
+    want, mass = R.rope_ref(x.view(n, H, r), ang, 1.0, r, layout)
+    tol = mass * (6.2832 * 2.0 ** -25 + 2.0 ** -23 + 3 * 2.0 ** -24)
+    err = (y.view(n, H, r).double().cpu() - want).abs()
     assert (err <= tol).all(), f"worst error / tolerance {float((err / tol).max())}"
 
 
