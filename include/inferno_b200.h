@@ -220,7 +220,9 @@ typedef struct InfernoRope {
   int32_t rope_dim;              /* even, 2..min(head_dim, 512) */
   int32_t layout;                /* INFERNO_ROPE_HALF / _INTERLEAVED */
   int32_t scaling;               /* INFERNO_ROPE_SCALE_* */
-  int32_t inverse;               /* 1: rotate back (also the gradient of the rotation) */
+  int32_t inverse;               /* 1: by the angles' negatives, cos and sin times the same factor: the
+                                  * gradient of the forward call.  To undo a forward call whose factor
+                                  * m is not 1, give mscale = 1 / m */
   int32_t orig_ctx;              /* scaling 2: positions of the unscaled context */
   int32_t n_rows;                /* rows of k_out / v_out that slots may name */
   float theta;                   /* > 1 */

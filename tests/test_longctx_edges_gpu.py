@@ -217,6 +217,38 @@ def test_rope_far_positions(theta, r, with_factors, layout):
     assert (err <= tol).all(), f"worst error / tolerance {float((err / tol).max())}"
 
 
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("scale", [dict(scaling=2, factor=8.0, orig_ctx=4096), dict(mscale=1.5)])
+def test_rope_inverse_with_a_gain(scale, layout):
+    """The inverse carries the forward call's factor m of cos and sin: it is the
+    gradient.  With mscale 1 / m it undoes the forward call."""
+    n, H, d, r = 5, 2, 64, 32
+    g = _gen(2)
+    w, x = torch.randn(n, H * d, generator=g, device="cuda"), torch.randn(n, H * d, generator=g, device="cuda")
+    pos = torch.tensor([0, 5, 90000, 77, 4095], dtype=torch.int32, device="cuda")
+    kw = dict(n_tokens=n, n_heads=H, n_kv_heads=0, head_dim=d, rope_dim=r, positions=pos, theta=1e4, layout=layout, **scale)
+    ang, m = R.rope_angles(pos, r, 1e4, **scale)
+    assert m != 1.0
+    # sincospi, the angle, m's own rounding and the products: 2^-21 of the pair's mass (see test_longctx_gpu.py)
+    got = torch.empty_like(w)
+    R.rope(R.rope_args(0, w, None, None, got, inverse=1, **kw))
+    want = torch.zeros(n, H, d, dtype=torch.float64)
+    wd = w.double().cpu().view(n, H, d)
+    for i in range(d):
+        unit = torch.zeros(n, H, d, dtype=torch.float64)
+        unit[..., i] = 1.0
+        up, down = R.rope_ref(unit, ang, m, r, layout)[0], R.rope_ref(-unit, ang, m, r, layout)[0]
+        want[..., i] = ((up - down) / 2 * wd).sum(-1)
+    _, mass = R.rope_ref(wd, ang, m, r, layout)
+    assert ((got.double().cpu().view(n, H, d) - want).abs() <= mass * 2.0 ** -21 + want.abs() * 2.0 ** -23).all()
+    y, z = torch.empty_like(x), torch.empty_like(x)
+    R.rope(R.rope_args(0, x, None, None, y, **kw))
+    R.rope(R.rope_args(0, y, None, None, z, inverse=1, **{**kw, "mscale": 1 / m}))
+    _, mass = R.rope_ref(x.view(n, H, d), ang, 1.0, r, layout)
+    # two rotations, the second of values of up to mass, and m 1 / m rounded
+    assert ((z - x).view(n, H, d).double().cpu().abs() <= mass * 2.0 ** -19 + 1e-30).all()
+
+
 # ---------------------------------------------------------------------------
 # waits that run out
 # ---------------------------------------------------------------------------
