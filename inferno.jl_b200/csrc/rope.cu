@@ -292,6 +292,8 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
   const bool has_q = r->n_heads > 0, has_k = r->n_kv_heads > 0 && r->k, has_v = r->v != nullptr;
   if (r->n_tokens == 0) return 0;
   if (!r->positions) return set_error(INFERNO_EINVAL, "rope: positions missing");
+  if (((uintptr_t)r->positions | (uintptr_t)r->slots | (uintptr_t)r->freq_factors) % 4)
+    return set_error(INFERNO_EINVAL, "rope: positions, slots or freq_factors is not aligned to 4 bytes");
   if (has_q && (!r->q || !r->q_out)) return set_error(INFERNO_EINVAL, "rope: q or q_out missing");
   if (has_k && !r->k_out) return set_error(INFERNO_EINVAL, "rope: k_out missing");
   if (has_v && (!r->slots || !r->v_out || r->n_kv_heads < 1))

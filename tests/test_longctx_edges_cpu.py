@@ -4,7 +4,7 @@ import ctypes as C
 
 import pytest
 
-from inferno_b200._lib import InfernoAttention, lib
+from inferno_b200._lib import InfernoAttention, InfernoRope, lib
 
 A = 0x10000            # addresses that are checked, never read
 STEP = 0x1000000
@@ -27,3 +27,13 @@ def test_attention_timeout_check_needs_a_kernel_that_waits(kw):
         assert rc == 0
     else:
         _refused(rc, "bounded waits")
+
+
+@pytest.mark.parametrize("field", ["positions", "slots", "freq_factors"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_rope_refuses_misaligned_indices(field, off):
+    a = InfernoRope(type=30, n_tokens=4, n_heads=8, n_kv_heads=2, head_dim=64, rope_dim=32, theta=1e4, positions=A,
+                    slots=A, n_rows=4, freq_factors=A, q=A + STEP, k=A + 2 * STEP, q_out=A + 3 * STEP, k_out=A + 4 * STEP,
+                    q_stride=512, k_stride=128, q_out_stride=512, k_out_stride=128)
+    setattr(a, field, A + off)
+    _refused(lib().inferno_rope(C.byref(a), None), "aligned")
