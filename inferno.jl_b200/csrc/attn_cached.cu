@@ -1435,7 +1435,9 @@ int ac_call(const InfernoAttention* a, void* workspace, int64_t workspace_bytes,
   if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < (int64_t)pl.bytes)
     return set_error(INFERNO_EINVAL, "attention_cached: workspace of %lld bytes, %lld needed (256-byte aligned)",
                      (long long)workspace_bytes, (long long)pl.bytes);
-  if ((rc = longctx_check_device(a->out, "attention_cached"))) return rc;
+  if ((rc = longctx_check_device({a->q, a->out, workspace}, "attention_cached"))) return rc;
+  if (a->prefix_len && (rc = longctx_check_device({a->prefix_k, a->prefix_v}, "attention_cached"))) return rc;
+  if (a->max_len && (rc = longctx_check_device({a->k_cache, a->v_cache, a->lens, a->scores}, "attention_cached"))) return rc;
   p.q = a->q;
   p.pk = a->prefix_k;
   p.pv = a->prefix_v;

@@ -469,7 +469,9 @@ extern "C" int inferno_cache_evict(const InfernoEvict* e, void* workspace, int64
   if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < evict_workspace(e))
     return set_error(INFERNO_EINVAL, "cache_evict: workspace of %lld bytes, %lld needed (256-byte aligned)",
                      (long long)workspace_bytes, (long long)evict_workspace(e));
-  if ((rc = longctx_check_device(e->k_cache, "cache_evict"))) return rc;
+  if ((rc = longctx_check_device({e->k_cache, e->v_cache, e->scores, e->slot_pos, e->lens, e->next_pos, e->scores_out,
+                                  e->slot_pos_out, e->lens_out, workspace}, "cache_evict")))
+    return rc;
   EvictParams p{};
   p.kc = (uint8_t*)e->k_cache;
   p.vc = (uint8_t*)e->v_cache;

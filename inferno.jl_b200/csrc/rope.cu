@@ -331,7 +331,7 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
         return set_error(INFERNO_EINVAL, "rope: %s_out overlaps %s", names[i], names[j]);
     }
   }
-  int rc = longctx_check_device(out[0].p ? out[0].p : out[1].p ? out[1].p : out[2].p, "rope");
+  int rc = longctx_check_device({in[0].p, in[1].p, in[2].p, out[0].p, out[1].p, out[2].p, r->positions, r->slots, r->freq_factors}, "rope");
   if (rc) return rc;
   const bool ilv = r->layout == INFERNO_ROPE_INTERLEAVED;
   long long all = (long long)r->head_dim * es | (long long)r->rope_dim * es;

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import longctx_ref as R
-from inferno_b200._lib import call, lib
+from inferno_b200._lib import InfernoError, call, lib
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -247,6 +247,67 @@ def test_rope_inverse_with_a_gain(scale, layout):
     _, mass = R.rope_ref(x.view(n, H, d), ang, 1.0, r, layout)
     # two rotations, the second of values of up to mass, and m 1 / m rounded
     assert ((z - x).view(n, H, d).double().cpu().abs() <= mass * 2.0 ** -19 + 1e-30).all()
+
+
+# ---------------------------------------------------------------------------
+# buffers that the device cannot read
+# ---------------------------------------------------------------------------
+def _calls():
+    """Valid calls of the three operators and what keeps their buffers alive."""
+    B, H, kv, d, L = 2, 4, 2, 64, 40
+    dev = dict(device="cuda")
+    x = {n: torch.zeros(B, 1, h, d, dtype=torch.bfloat16, **dev) for n, h in (("q", H), ("out", H), ("k", kv), ("v", kv))}
+    x.update({n: torch.zeros(B, L, kv, d, dtype=torch.bfloat16, **dev) for n in ("kc", "vc")})
+    x.update({n: torch.zeros(20, kv, d, dtype=torch.bfloat16, **dev) for n in ("pk", "pv")})
+    x.update({n: torch.zeros(B, kv, L, **dev) for n in ("scores", "scores_out")})
+    x.update({n: torch.zeros(B, kv, L, dtype=torch.int32, **dev) for n in ("pos", "pos_out")})
+    x.update({n: torch.full((B,), 30, dtype=torch.int32, **dev) for n in ("lens", "next_pos", "lens_out", "slots")})
+    x["slots"][1] = 70
+    x["ff"] = torch.ones(d // 2, **dev)
+    rope = R.rope_args(30, x["q"].view(B, -1), x["k"].view(B, -1), x["v"].view(B, -1), x["out"].view(B, -1),
+                       x["kc"].view(B * L, -1), x["vc"].view(B * L, -1), n_tokens=B, n_heads=H, n_kv_heads=kv, head_dim=d,
+                       rope_dim=d, positions=x["lens"], theta=1e4, slots=R.ptr(x["slots"]), n_rows=B * L,
+                       freq_factors=R.ptr(x["ff"]))
+    attn = R.attention_args(30, x["q"], x["out"], x["lens"], x["kc"], x["vc"], x["pk"], x["pv"], x["scores"])
+    evict = R.evict_args(30, x["kc"], x["vc"], x["scores"], x["pos"], x["lens"], x["next_pos"], x["scores_out"],
+                         x["pos_out"], x["lens_out"], budget=16)
+    x["ws"] = torch.empty(max(R.attention_workspace(attn).numel(), R.evict_workspace(evict).numel()), dtype=torch.uint8, **dev)
+    ws, n = C.c_void_p(x["ws"].data_ptr()), x["ws"].numel()
+    return x, {"inferno_rope": (rope, lambda a: ()), "inferno_attention_cached": (attn, lambda a: (ws, n)),
+               "inferno_cache_evict": (evict, lambda a: (ws, n))}
+
+
+@pytest.mark.parametrize("fn,fields", [
+    ("inferno_rope", "q k v q_out k_out v_out positions slots freq_factors"),
+    ("inferno_attention_cached", "q out prefix_k prefix_v k_cache v_cache lens scores"),
+    ("inferno_cache_evict", "k_cache v_cache scores slot_pos lens next_pos scores_out slot_pos_out lens_out")])
+def test_any_buffer_in_host_memory_is_refused(fn, fields):
+    _, calls = _calls()
+    a, more = calls[fn]
+    host = torch.zeros(1 << 16)
+    call(fn, C.byref(a), *more(a), R.stream())
+    for field in fields.split():
+        good = getattr(a, field)
+        setattr(a, field, host.data_ptr())
+        with pytest.raises(InfernoError, match="not device memory"):
+            call(fn, C.byref(a), *more(a), R.stream())
+        setattr(a, field, good)
+    if fn != "inferno_rope":
+        size = getattr(lib(), fn + "_workspace")(C.byref(a))
+        store = torch.zeros(size + 256, dtype=torch.uint8)
+        at = (store.data_ptr() + 255) // 256 * 256
+        with pytest.raises(InfernoError, match="not device memory"):
+            call(fn, C.byref(a), C.c_void_p(at), size, R.stream())
+    call(fn, C.byref(a), *more(a), R.stream())
+
+
+def test_pinned_lengths_are_read():
+    """Pinned host memory is memory of CUDA's, which a kernel can read."""
+    tid, c = _case("bf16", 3, 1, 4, 2, 64, 40, [90, 33, 1], seed=2)
+    out, scores = _run(tid, c)
+    got, got_scores = _run(tid, dict(c, lens=c["lens"].cpu().pin_memory()))
+    torch.cuda.synchronize()
+    assert torch.equal(got, out) and torch.equal(got_scores, scores)
 
 
 # ---------------------------------------------------------------------------
