@@ -311,6 +311,29 @@ def test_pinned_lengths_are_read():
 
 
 # ---------------------------------------------------------------------------
+# what the next position protects
+# ---------------------------------------------------------------------------
+def test_evict_protects_the_recent_rows_before_the_next_position():
+    """A decode step that advances its positions before it evicts keeps its first
+    n_sink and last n_recent rows, and no other where the budget has no more; with the
+    positions of the tokens just appended one row more is protected, and the rows of
+    both kinds, now more than the budget, compete by weight."""
+    B, kv, L, sink, recent = 2, 2, 60, 3, 9
+    k, v = (torch.zeros(B, L, kv, 64, device="cuda") for _ in range(2))
+    scores = torch.arange(L, 0, -1, device="cuda").float().expand(B, kv, L).contiguous()      # the newest weigh least
+    pos = torch.arange(L, device="cuda", dtype=torch.int32).expand(B, kv, L).contiguous()
+    for ahead, kept in ((0, list(range(sink)) + list(range(L - recent, L))),
+                        (-1, list(range(sink)) + list(range(L - recent - 1, L - 1)))):
+        lens = torch.full((B,), L, dtype=torch.int32, device="cuda")
+        nxt = torch.full((B,), L + ahead, dtype=torch.int32, device="cuda")
+        so, po, lo = torch.zeros_like(scores), torch.zeros_like(pos), torch.zeros_like(lens)
+        R.evict(R.evict_args(0, k, v, scores, pos, lens, nxt, so, po, lo, budget=sink + recent, n_sink=sink, n_recent=recent))
+        for b in range(B):
+            for h in range(kv):
+                assert sorted(po[b, h, :sink + recent].tolist()) == kept
+
+
+# ---------------------------------------------------------------------------
 # waits that run out
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype,B,H,kv,d,P", [("bf16", 24, 8, 2, 128, 3000), ("f16", 24, 8, 2, 64, 6000),
