@@ -256,7 +256,13 @@ int inferno_rope(const InfernoRope* r, void* stream);
  * as infinite.)
  * scores (optional, fp32): scores[(b * n_kv_heads + h) * score_stride + j]
  * gains the weight that own row j got, summed over the tokens and query heads
- * of KV head h; entries from lens[b] on are left as they are.
+ * of KV head h; entries from lens[b] on are left as they are.  V does not enter
+ * them.  Tokens that are padding add theirs like any other: a call that has
+ * such tokens is made without scores.
+ * The 16-bit types round each p_j (before its division by the sum) to the type
+ * for the product with V: half a step of each weight, as much as the output's
+ * own rounding; fp16 weights below 2^-25 of the largest round in fixed steps of
+ * at most 2^-35 of it.  The sum takes them unrounded.
  * q and out [batch * n_tokens][n_heads][head_dim] with q_stride / out_stride
  * elements between token rows; out may be q, and overlaps nothing else.
  * head_dim 64, 128 or 256; pointers and strides multiples of 16 bytes (lens and
