@@ -15,7 +15,8 @@
 // written, so the CTAs of the cluster move K and V in any order.
 //
 // Bound: the bytes of the rows that move (read and written), after a chain of
-// up to six cluster barriers that few rows cannot hide.
+// up to seven cluster barriers (four digits, the first once more where the rows kept
+// always exceed the budget, the ties, the lists) that few rows cannot hide.
 #include <algorithm>
 #include <cooperative_groups.h>
 #include "internal.h"
@@ -43,7 +44,7 @@ struct EvictParams {
   const int* pos;
   const int *lens, *next_pos;
   float* scores_out;
-  int *pos_out, *lens_out;            // lens_out null: written by evict_lens_kernel
+  int *pos_out, *lens_out;            // lens_out null: written by evict_move_kernel
   long long stride;                   // entries between (sequence, KV head) rows of scores / pos
   int nkv, max_len, budget, n_sink, n_recent, max_moves;
   int words;                          // 32-row words a CTA's part may have
