@@ -39,18 +39,17 @@ constexpr int AC_KT = 16;                       // keys per tile
 constexpr int AC_SMEM = 227 * 1024, AC_SMEM_HALF = 112 * 1024;
 constexpr int AC_FIN_THREADS = 256;
 
-// P_EXP: P is taken times 2^P_EXP, and so are its sum and O (a part's "largest logit"
-// is that much smaller, so joining parts needs no more).  fp16 has its full precision
-// down to 2^-14 only, and nothing below 2^-25: with the largest weight at 2^15 that is
-// 2^-29 and 2^-40 of it, so that a long tail of small weights is not lost.
+// P_EXP: log2 of the largest P (ac_ref); sum and O are scaled alike.  fp16 has its full
+// precision down to 2^-14 only, and nothing below 2^-25: with the largest weight at
+// 2^15 that is 2^-29 and 2^-40 of it, so that a long tail of small weights is not lost.
 template <typename T>
 struct AcType;
 template <>
-struct AcType<float> { static constexpr bool F32 = true; static constexpr float P_EXP = 0.f; };
+struct AcType<float> { static constexpr bool F32 = true; static constexpr int P_EXP = 0; };
 template <>
-struct AcType<__half> { static constexpr bool F32 = false; static constexpr float P_EXP = 15.f; };
+struct AcType<__half> { static constexpr bool F32 = false; static constexpr int P_EXP = 15; };
 template <>
-struct AcType<__nv_bfloat16> { static constexpr bool F32 = false; static constexpr float P_EXP = 0.f; };
+struct AcType<__nv_bfloat16> { static constexpr bool F32 = false; static constexpr int P_EXP = 0; };
 
 // geometry of one instantiation
 template <typename T, int HD, int R>
@@ -563,16 +562,17 @@ __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork 
 #pragma unroll
       for (int n = 0; n < 2; ++n) *(float2*)(lg_hi + key0 + 8 * n + 2 * t4) = make_float2(s[n][2], s[n][3]);
     }
+    constexpr int PE = AcType<T>::P_EXP;
     if (__any_sync(0xffffffffu, mx_lo > m_lo || mx_hi > m_hi)) {
       const float n_lo = fmaxf(m_lo, mx_lo), n_hi = fmaxf(m_hi, mx_hi);
-      const float f_lo = n_lo == -INFINITY ? 1.f : exp2f(m_lo - n_lo), f_hi = n_hi == -INFINITY ? 1.f : exp2f(m_hi - n_hi);
+      const float f_lo = n_lo == -INFINITY ? 1.f : exp2f(ac_ref<PE>(m_lo) - ac_ref<PE>(n_lo));
+      const float f_hi = n_hi == -INFINITY ? 1.f : exp2f(ac_ref<PE>(m_hi) - ac_ref<PE>(n_hi));
       m_lo = n_lo, m_hi = n_hi;
       l_lo *= f_lo, l_hi *= f_hi;
 #pragma unroll
       for (int x = 0; x < HD / 8; ++x) o[x][0] *= f_lo, o[x][1] *= f_lo, o[x][2] *= f_hi, o[x][3] *= f_hi;
     }
-    constexpr float PE = AcType<T>::P_EXP;
-    const float z_lo = m_lo == -INFINITY ? 0.f : m_lo - PE, z_hi = m_hi == -INFINITY ? 0.f : m_hi - PE;
+    const float z_lo = m_lo == -INFINITY ? 0.f : ac_ref<PE>(m_lo), z_hi = m_hi == -INFINITY ? 0.f : ac_ref<PE>(m_hi);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -667,8 +667,8 @@ __device__ __forceinline__ void ac_part_segment(const AcParams& p, const AcWork 
   }
 
   // ---- merge the key groups ----
-  m_lo -= AcType<T>::P_EXP;
-  m_hi -= AcType<T>::P_EXP;
+  m_lo = ac_ref<AcType<T>::P_EXP>(m_lo);
+  m_hi = ac_ref<AcType<T>::P_EXP>(m_hi);
 #pragma unroll
   for (int of = 1; of <= 2; of <<= 1) {
     l_lo += __shfl_xor_sync(0xffffffffu, l_lo, of);

@@ -8,9 +8,9 @@
 namespace inf {
 
 // Query rows are numbered r = (b * n_tokens + t) * n_heads + h.  A CTA leaves, for
-// each of its rows, one partial result over its keys: the largest logit (less a
-// constant of the kernel and type) and the sum and weighted V sum of exp2(logit -
-// that); logits are in units of log2.
+// each of its rows, one partial result over its keys: the largest logit (or a reference
+// near it, below) and the sum and weighted V sum of exp2(logit - that); logits are in
+// units of log2.
 //
 // The prefix is cut into p_splits equal splits; row r's partial of split s is entry
 // r * p_splits + s.  The own parts are cut evenly whatever lens are: keys are counted
@@ -42,6 +42,15 @@ struct AcParams {
   float* logits;                 // [row][logit_stride] own logits (only with scores)
   long long logit_stride;
 };
+
+// What a row's logits are taken relative to when the largest is `top`: that less `exp`,
+// so that the largest P is 2^exp.  From 2^22 on, where fp32 has no room for the
+// difference, top itself.
+constexpr float AC_FAR = 4194304.f;
+template <int exp>
+__device__ __forceinline__ float ac_ref(float top) {
+  return exp && fabsf(top) < AC_FAR ? top - (float)exp : top;
+}
 
 constexpr int AC_BLOCK = 64;
 constexpr float AC_LOG2E = 1.4426950408889634f;

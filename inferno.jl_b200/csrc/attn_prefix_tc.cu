@@ -5,12 +5,12 @@
 // A CTA takes 128 query rows of one KV head against one split of the prefix, in
 // tiles of 64 keys:
 //   S = Q K^T   A = Q tile, B = K tile in shared memory, S in TMEM (two buffers)
-//   P = exp2(scale S - m), rounded to the 16-bit type (half a step of each weight, as
+//   P = exp2(scale S - r), rounded to the 16-bit type (half a step of each weight, as
 //   in attn_cached.cu; the sum takes it unrounded), back into S's columns
 //   O += P V    A = P in TMEM, B = V tile, N-major as it lies in the cache
-// Warps 0-3: softmax, one thread per row (TMEM lane); the running maximum is
-// raised, and O rescaled, only when a row outgrows it by 2^8 (fp16 2^4), since P and
-// the sums hold that much headroom.  Warp 4: K and V tiles by TMA.  Warp 5: issues the
+// Warps 0-3: softmax, one thread per row (TMEM lane); r, the reference of a row, follows
+// its running maximum, and O is rescaled, only when that outgrows it by 2^8 (fp16 2^4),
+// since P and the sums hold that much headroom.  Warp 4: K and V tiles by TMA.  Warp 5: issues the
 // MMAs; S of the next tile is issued before P V of this one.  Two CTAs per SM (one at
 // head_dim 256) fill each other's gaps.
 //
@@ -36,15 +36,15 @@ namespace {
 constexpr int AP_M = 128, AP_N = 64;
 constexpr int AP_THREADS = 192;
 
-// SLACK: log2 of what P may exceed the value at the running maximum by, before that is
-// raised.  P_EXP: log2 of P at the running maximum; sum and O are scaled alike, and the
-// part's "largest logit" is that much smaller.  fp16 has its full precision down to
-// 2^-14 only, and nothing below 2^-25: 2^11 at the maximum and 2^15 at most leave it
-// down to 2^-25 (and something down to 2^-36) of the maximum.
+// P_EXP: log2 of P at the maximum when the reference was set (ac_ref); sum and O are
+// scaled alike.  SLACK: log2 of what P may exceed that by before the reference is
+// raised.  fp16 has its full precision down to 2^-14 only, and nothing below 2^-25:
+// 2^11 at the maximum and 2^15 at most leave it down to 2^-25 (and something down to
+// 2^-36) of the maximum.
 template <typename T>
-struct ApType { static constexpr float SLACK = 8.f, P_EXP = 0.f; };
+struct ApType { static constexpr int P_EXP = 0; static constexpr float SLACK = 8.f; };
 template <>
-struct ApType<__half> { static constexpr float SLACK = 4.f, P_EXP = 11.f; };
+struct ApType<__half> { static constexpr int P_EXP = 11; static constexpr float SLACK = 4.f; };
 
 template <int HD>
 struct ApGeo {
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
     mbar_arrive(q_full);
 
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    float m = -INFINITY, l = 0.f;
+    float ref = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       ok = ap_wait(&s_full[j & 1], (j >> 1) & 1, polls);
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
           if (i + 32 < live) u1[i] ^= 0x80000000u;
         }
       }
-      const float sc = fabsf(p.scale_log2);
+      float sc = fabsf(p.scale_log2);
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         mx[0] = fmaxf(mx[0], __uint_as_float(u0[i]));
@@ -317,7 +317,19 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         mx[3] = fmaxf(mx[3], __uint_as_float(u1[i + 1]));
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-      const bool raise = j == 0 || top > m + ApType<T>::SLACK;
+      // one rounding of scale S - r below leaves half a step of a far logit in P: such
+      // rows are scaled, and so rounded, first
+      if (fabsf(top) >= AC_FAR) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          u0[i] = __float_as_uint(__uint_as_float(u0[i]) * sc);
+          u1[i] = __float_as_uint(__uint_as_float(u1[i]) * sc);
+        }
+        sc = 1.f;
+      }
+      constexpr int PE = ApType<T>::P_EXP;
+      const float room = (PE && fabsf(ref) < AC_FAR ? (float)PE : 0.f) + ApType<T>::SLACK;
+      const bool raise = j == 0 || top - ref > room;
       if (j > 0 && __any_sync(0xffffffffu, raise)) {
         // O holds P V up to tile j - 1 once that is done (j - 2 was before S (j) was
         // issued); P V (j) waits for this thread
@@ -327,7 +339,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
           break;
         }
         tc_fence_after();
-        const float f = raise ? ex2(m - top) : 1.0f;    // m = -inf: nothing gathered yet, f = 0
+        const float f = raise ? ex2(ref - ac_ref<PE>(top)) : 1.0f;    // ref = -inf: nothing gathered yet, f = 0
         l *= f;
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
@@ -340,8 +352,8 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
         }
         tmem_wait_st();
       }
-      if (raise) m = top;
-      const float z = m == -INFINITY ? 0.f : m - ApType<T>::P_EXP;
+      if (raise) ref = ac_ref<PE>(top);
+      const float z = ref == -INFINITY ? 0.f : ref;
       float sum[2] = {0.f, 0.f};
       uint32_t pk[32];
 #pragma unroll
@@ -400,7 +412,7 @@ __global__ void __launch_bounds__(AP_THREADS, ApGeo<HD>::CTAS) ap_kernel(const _
       if (r < nrows) {
         int tok, h;
         ap_row(p, kvh, r, tok, h);
-        p.part_ml[((long long)tok * p.nh + h) * p.p_splits + split] = make_float2(m - ApType<T>::P_EXP, l);
+        p.part_ml[((long long)tok * p.nh + h) * p.p_splits + split] = make_float2(ref, l);
       }
     } else if (row0 + tid < nrows) {
       int tok, h;

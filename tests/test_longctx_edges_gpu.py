@@ -173,6 +173,31 @@ def test_attention_small_weights_add_up(dtype, weight, B, H, d, P, lens):
     assert (err <= tol).all(), f"worst error / tolerance {float((err / tol).max())}"
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("B,H,d,P,lens", [
+    (1, 4, 64, 0, [777]), (1, 20, 128, 0, [333]), (1, 40, 256, 0, [100]), (2, 4, 128, 1000, [1, 1]),
+    (16, 4, 64, 16001, [1] * 16), (16, 4, 128, 4097, [1] * 16), (16, 4, 256, 3001, [1] * 16)])
+def test_attention_huge_logits(dtype, B, H, d, P, lens):
+    """Logits of up to 1e8 (and, scaled, 1e10), whose steps in fp32 are 8 and more: the
+    largest takes all the weight, the others being thousands below, and the output is
+    its V: bit for bit in 16 bits, in fp32 to the 2^-19 that the pair products keep."""
+    tid, c = _case(dtype, B, 1, H, 1, d, P, lens, seed=10)
+    for n in ("q", "k", "pk"):
+        if n in c:
+            c[n].copy_(torch.randint(-7, 8, c[n].shape, generator=_gen(len(n)), device="cuda") * 1000.0)
+    c.pop("scores")
+    for scale in (d ** -0.5, -100.0):
+        R.attention(R.attention_args(tid, scale=scale, **c))
+        for b, n in enumerate(lens):
+            keys = torch.cat([c["pk"][:, 0], c["k"][b, :n, 0]] if P else [c["k"][b, :n, 0]]).double()
+            vals = torch.cat([c["pv"][:, 0], c["v"][b, :n, 0]] if P else [c["v"][b, :n, 0]])
+            top = (c["q"][b, 0].double() @ keys.t() * scale).topk(2, -1)
+            sure = top.values[:, 0] - top.values[:, 1] > 1e4
+            assert sure.any()
+            got, want = c["out"][b, 0][sure], vals[top.indices[:, 0]][sure]
+            assert torch.equal(got, want) if dtype != "f32" else ((got - want).abs() <= want.abs() * 2.0 ** -19).all()
+
+
 # ---------------------------------------------------------------------------
 # far positions
 # ---------------------------------------------------------------------------
