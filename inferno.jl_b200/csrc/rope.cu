@@ -10,12 +10,13 @@
 // instructions: 96 us for 16383 tokens x 40 heads of 128 bf16, and more items in
 // flight only made it slower.)
 //
-// Angles: f_i / (2 pi) is a double and a rest, 2^-54 of itself off at most (see the
-// host), and its product with the position is taken exactly, the double's and the
-// rest's; the whole turns are dropped in double and what is left, at most half a
-// turn, goes to sincospi in fp32.  Up to 2^28.4 turns (position 2^31 - 1) the angle
-// is off by 2 pi (2^-26 + 2^-26), 2e-7, from the frequency and from its rounding to
-// fp32; by half of that up to position 2^28.
+// Angles: f_i / (2 pi), the turns per position, is a 64-bit fraction, so its product
+// with the position modulo 2^64 is the fraction of a turn that is left, whole turns
+// dropped; that goes to sincospi in fp32.  The frequency is off by 2^-54 of itself (see
+// the host) and 2^-64, so up to position 2^31 - 1 (2^28.4 turns) the angle is off by
+// 2 pi (2^-26 + 2^-26), 2e-7, from it and from the rounding to fp32; by half of that up
+// to position 2^28.  With freq_factors the frequency, in 64 bits of a unit of its own, is
+// taken apart into a double and its rest, divided by the factor and multiplied exactly.
 //
 // Bound: bytes, each value read and written once.
 #include <algorithm>
@@ -48,8 +49,10 @@ struct RopeParams {
   uint32_t v_slice;                      // v vectors of one block (over its tb tokens)
   FastDiv by_units, by_v;
   float gain, sign;                      // factor of cos and sin; -1: rotate back
-  double turns[ROPE_MAX_PAIRS];          // f_i / (2 pi), without freq_factors
-  float turns_rest[ROPE_MAX_PAIRS];      // what the double leaves of it
+  // f_i / (2 pi) times 2^64, modulo 2^64; with freq_factors not divided by them, and not
+  // modulo 2^64 but in `unit`
+  unsigned long long turns[ROPE_MAX_PAIRS];
+  double unit;
 };
 
 template <typename T, int V>
@@ -101,6 +104,15 @@ __host__ __device__ constexpr int rope_heads() {
   return V == 8 && !ILV ? 2 : 4;
 }
 
+// half turns, less whole turns, of a pair with a factor w at a position
+__device__ __forceinline__ float rope_half_turns(unsigned long long turns, double unit, double w, double at) {
+  const double f = (double)(turns & ~0x7ffull) * unit, f_rest = (double)(turns & 0x7ffull) * unit;
+  const double inv = 1.0 / w, g = f * inv;
+  const double rest = g == 0.0 ? 0.0 : (fma(-g, w, f) + f_rest) * inv;       // 0: an infinite factor
+  const double turn = g * at;
+  return 2.0f * (float)(turn - rint(turn) + (fma(g, at, -turn) + rest * at));
+}
+
 // V: elements of one access (the widest that sizes, strides and pointers
 // allow).  ILV: interleaved pairs; a column then holds whole pairs.
 template <typename T, int V, bool ILV>
@@ -114,18 +126,19 @@ __global__ void __launch_bounds__(ROPE_THREADS, 4) rope_kernel(const __grid_cons
   const int t0 = blockIdx.x * p.tb, nt = min(p.tb, p.n_tokens - t0);
   for (int i = threadIdx.x; i < nt * half; i += ROPE_THREADS) {
     const int t = i / half, c = i - t * half;
-    double f = p.turns[c], rest = p.turns_rest[c];
-    if (p.freq_factors) {
-      const double w = __ldg(p.freq_factors + c), g = f / w;
-      rest = (fma(-g, w, f) + rest) / w;
-      f = g;
+    const int pos = __ldg(p.positions + t0 + t);
+    // as a double it is one load of a constant, whose lanes differ and go one by one; as
+    // an integer two, and every call 0.15 us longer
+    const unsigned long long turns = __double_as_longlong(((const double*)p.turns)[c]);
+    float half_turns;
+    if (!p.freq_factors) {
+      const unsigned long long left = turns * (unsigned long long)(long long)pos + 0x80000000ull;
+      half_turns = (float)(int)(left >> 32) * 0x1p-31f;            // rounded to 2^-32 turns
+    } else {
+      half_turns = rope_half_turns(turns, p.unit, __ldg(p.freq_factors + c), pos);
     }
-    const double at = __ldg(p.positions + t0 + t);
-    double turn = f * at;
-    rest = fma(f, at, -turn) + rest * at;
-    turn = turn - rint(turn) + rest;
     float sn, cn;
-    sincospif(2.0f * (float)turn, &sn, &cn);
+    sincospif(half_turns, &sn, &cn);
     cs[i] = make_float2(cn * p.gain, sn * p.gain * p.sign);
   }
   __syncthreads();
@@ -396,8 +409,16 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
       const long double ramp = std::min(std::max((i - low) / std::max(high - low, 0.001), 0.0), 1.0);
       g = f * (1.0L - ramp) + f / r->factor * ramp;
     }
-    p.turns[i] = (double)g;
-    p.turns_rest[i] = (float)(g - (long double)p.turns[i]);
+    if (p.freq_factors) {
+      if (i == 0) {                      // the largest: 64 bits of it
+        int e;
+        std::frexp(g, &e);
+        p.unit = std::ldexp(1.0, e - 64);
+      }
+      p.turns[i] = (unsigned long long)(g / p.unit);
+    } else {
+      p.turns[i] = (unsigned long long)((g < 1.0L ? g : g - std::floor(g)) * 0x1p64L);
+    }
   }
 
   // tokens per block: about four units for every team, fewer when there are too

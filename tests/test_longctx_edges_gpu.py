@@ -243,6 +243,47 @@ def test_rope_far_positions(theta, r, with_factors, layout):
 
 
 @pytest.mark.parametrize("layout", [0, 1])
+def test_rope_infinite_factor_and_negative_positions(layout):
+    """A pair whose factor is infinite does not turn; a negative position turns back,
+    with factors and without (the same angle, so the same bits)."""
+    n, r = 4, 32
+    g = _gen(13)
+    x = torch.randn(n, r, generator=g, device="cuda")
+    pos = torch.tensor([1, 77, 123456, 1 << 30], dtype=torch.int32, device="cuda")
+    ff = torch.full((r // 2,), INF, device="cuda")
+    kw = dict(n_tokens=n, n_heads=1, n_kv_heads=0, head_dim=r, rope_dim=r, theta=1e4, layout=layout)
+    y, z = torch.empty_like(x), torch.empty_like(x)
+    R.rope(R.rope_args(0, x, None, None, y, positions=pos, freq_factors=R.ptr(ff), **kw))
+    assert torch.equal(y, x)
+    for f in (None, torch.full_like(ff, 1.25)):
+        R.rope(R.rope_args(0, x, None, None, y, positions=pos, inverse=1, freq_factors=R.ptr(f), **kw))
+        R.rope(R.rope_args(0, x, None, None, z, positions=-pos, freq_factors=R.ptr(f), **kw))
+        assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("with_factors", [False, True])
+@pytest.mark.parametrize("theta", [1.1, 1e4])
+def test_rope_more_than_a_turn_per_position(theta, with_factors):
+    """A factor below 1 / (2 pi) gives pairs of more than one turn per position.  20
+    turns times 5000 positions are exact to 2^-36 in either form, so the tolerance is
+    that of the fp32 steps: 2 pi 2^-26 in the angle, 2^-23, 3 * 2^-24; the plain form's
+    angles of up to 7e5 are off by 2^-33."""
+    n, r = 6, 64
+    g = _gen(14)
+    x = torch.randn(n, r, generator=g, device="cuda")
+    pos = torch.tensor([0, 1, 2, 999, 4321, 5000], dtype=torch.int32, device="cuda")
+    ff = torch.rand(r // 2, generator=g, device="cuda") + 0.5 if with_factors else None
+    y = torch.empty_like(x)
+    R.rope(R.rope_args(0, x, None, None, y, n_tokens=n, n_heads=1, n_kv_heads=0, head_dim=r, rope_dim=r, positions=pos,
+                       theta=theta, scaling=1, factor=0.0078125, freq_factors=R.ptr(ff)))
+    theta = float(torch.tensor(theta))                         # as the struct holds it
+    ang, _ = R.rope_angles(pos, r, theta, scaling=1, factor=0.0078125, freq_factors=ff)
+    want, mass = R.rope_ref(x.view(n, 1, r), ang, 1.0, r, 0)
+    err = (y.view(n, 1, r).double().cpu() - want).abs()
+    assert (err <= mass * (6.2832 * 2.0 ** -26 + 2.0 ** -23 + 3 * 2.0 ** -24 + 2.0 ** -30)).all()
+
+
+@pytest.mark.parametrize("layout", [0, 1])
 @pytest.mark.parametrize("scale", [dict(scaling=2, factor=8.0, orig_ctx=4096), dict(mscale=1.5)])
 def test_rope_inverse_with_a_gain(scale, layout):
     """The inverse carries the forward call's factor m of cos and sin: it is the
