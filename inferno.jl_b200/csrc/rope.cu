@@ -5,10 +5,10 @@
 // positions[t] * f_i.  A block takes a few tokens: its threads first put cos and
 // sin of the tokens' angles into shared memory, once for all heads.  Then a team
 // of threads, one per 16-byte column of a head (a column of the half layout is two
-// vectors, rope_dim / 2 apart), takes four heads (or two) of a token at a time: cos and sin
-// of a column are read once for them, and the loads of all are in flight together.  (One vector per thread and index computation was bound by
-// instructions: 96 us for 16383 tokens x 40 heads of 128 bf16, and more items in
-// flight only made it slower.)
+// vectors, rope_dim / 2 apart), takes four heads (or two) of a token at a time: cos and
+// sin of a column are read once for them, and the loads of all are in flight together.
+// (One vector per thread and index computation was bound by instructions: 96 us for
+// 16383 tokens x 40 heads of 128 bf16, and more items in flight only made it slower.)
 //
 // Angles: f_i / (2 pi), the turns per position, is a 64-bit fraction, so its product
 // with the position modulo 2^64 is the fraction of a turn that is left, whole turns
