@@ -402,6 +402,11 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
     high = std::min(std::ceil(dim(slow)), r->rope_dim - 1.0);
   }
   long double f = 1.0L / 6.283185307179586476925286766559005768L;
+  // 64 bits of the largest, which is not the first pair's where parts are made faster
+  int unit_exp;
+  std::frexp(r->scaling == INFERNO_ROPE_SCALE_LINEAR || (r->scaling == INFERNO_ROPE_SCALE_PARTS && r->factor < 1.0f) ? f / r->factor : f,
+             &unit_exp);
+  p.unit = std::ldexp(1.0, unit_exp - 64);
   for (int i = 0; i < half; ++i, f *= ratio) {
     long double g = f;
     if (r->scaling == INFERNO_ROPE_SCALE_LINEAR) g = f / r->factor;
@@ -410,11 +415,6 @@ extern "C" int inferno_rope(const InfernoRope* r, void* stream) {
       g = f * (1.0L - ramp) + f / r->factor * ramp;
     }
     if (p.freq_factors) {
-      if (i == 0) {                      // the largest: 64 bits of it
-        int e;
-        std::frexp(g, &e);
-        p.unit = std::ldexp(1.0, e - 64);
-      }
       p.turns[i] = (unsigned long long)(g / p.unit);
     } else {
       p.turns[i] = (unsigned long long)((g < 1.0L ? g : g - std::floor(g)) * 0x1p64L);

@@ -283,6 +283,26 @@ def test_rope_more_than_a_turn_per_position(theta, with_factors):
     assert (err <= mass * (6.2832 * 2.0 ** -26 + 2.0 ** -23 + 3 * 2.0 ** -24 + 2.0 ** -30)).all()
 
 
+@pytest.mark.parametrize("with_factors", [False, True])
+@pytest.mark.parametrize("factor,orig_ctx", [(0.125, 8), (0.0078125, 30), (0.5, 4096)])
+def test_rope_by_parts_with_a_factor_below_one(factor, orig_ctx, with_factors):
+    """Later pairs then turn faster than the first.  Tolerance as above, with 7e5 of
+    angle at most."""
+    n, r = 6, 64
+    g = _gen(15)
+    x = torch.randn(n, r, generator=g, device="cuda")
+    pos = torch.tensor([0, 1, 2, 999, 4321, 5000], dtype=torch.int32, device="cuda")
+    ff = torch.rand(r // 2, generator=g, device="cuda") + 0.5 if with_factors else None
+    y = torch.empty_like(x)
+    kw = dict(scaling=2, factor=factor, orig_ctx=orig_ctx)
+    R.rope(R.rope_args(0, x, None, None, y, n_tokens=n, n_heads=1, n_kv_heads=0, head_dim=r, rope_dim=r, positions=pos,
+                       theta=1e4, freq_factors=R.ptr(ff), **kw))
+    ang, gain = R.rope_angles(pos, r, 1e4, freq_factors=ff, **kw)
+    want, mass = R.rope_ref(x.view(n, 1, r), ang, gain, r, 0)
+    err = (y.view(n, 1, r).double().cpu() - want).abs()
+    assert (err <= mass * (6.2832 * 2.0 ** -26 + 2.0 ** -23 + 3 * 2.0 ** -24 + 2.0 ** -30)).all()
+
+
 @pytest.mark.parametrize("layout", [0, 1])
 @pytest.mark.parametrize("scale", [dict(scaling=2, factor=8.0, orig_ctx=4096), dict(mscale=1.5)])
 def test_rope_inverse_with_a_gain(scale, layout):
